@@ -1244,3 +1244,5 @@ extern "C" int b200_block_forward_noalloc(const B200BlockArgs* args, b200_stream
   a.workspace_bytes = B200_NOALLOC_SCRATCH_BYTES;
   return block_impl(&a, static_cast<cudaStream_t>(stream));
 }
+
+#include "serving_host.cuh"

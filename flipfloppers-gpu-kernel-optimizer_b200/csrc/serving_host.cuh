@@ -1,0 +1,279 @@
+// Host side of the 8-bit serving operators: argument checks and launches.  Part of
+// the library's one translation unit (included by b200_block.cu, whose helpers it uses).
+#pragma once
+
+#include "attn8.cuh"
+#include "gemm_i8.cuh"
+
+namespace {
+
+int cache8_check(const B200KvCache8* c) {
+  if (!c || !c->k_pages || !c->v_pages || !c->k_scale || !c->v_scale || !c->k_newest || !c->v_newest || !c->table)
+    return B200_ERR_ARG;
+  if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return B200_ERR_HEAD_DIM;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return B200_ERR_TILE;
+  if (c->batch <= 0 || c->kv_heads <= 0 || c->num_pages <= 0 || c->newest_rows <= 0 || c->table_width <= 0)
+    return B200_ERR_ARG;
+  if (c->batch > ATTN8_MAX_BATCH || c->kv_heads > 1024) return B200_ERR_TILE;
+  // positions are numbered in 32 bits
+  if (static_cast<long long>(c->table_width) * c->page_size > 0x7fff0000LL) return B200_ERR_TILE;
+  if (!al16(c->k_pages) || !al16(c->v_pages) || !al16(c->k_newest) || !al16(c->v_newest)) return B200_ERR_ALIGN;
+  return B200_OK;
+}
+
+Kv8Cache cache8_of(const B200KvCache8* a) {
+  Kv8Cache c{};
+  c.k_pages = static_cast<uint8_t*>(a->k_pages);
+  c.v_pages = static_cast<uint8_t*>(a->v_pages);
+  c.k_scale = a->k_scale;
+  c.v_scale = a->v_scale;
+  c.k_new = static_cast<uint16_t*>(a->k_newest);
+  c.v_new = static_cast<uint16_t*>(a->v_newest);
+  c.table = a->table;
+  c.rows = a->rows;
+  c.num_pages = a->num_pages;
+  c.kv_heads = a->kv_heads;
+  c.page = a->page_size;
+  c.head_dim = a->head_dim;
+  c.new_rows = a->newest_rows;
+  c.table_width = a->table_width;
+  c.bf16 = a->bf16 != 0;
+  return c;
+}
+
+int kv8_append_impl(const B200KvCache8* c, const void* qkv, long long ld, void* q_out, const int* cu, const int* start,
+                    const float* cos, const float* sin, int rot, int interleaved, int rope_rows, int tokens, int heads,
+                    cudaStream_t st) {
+  if (int rc = cache8_check(c)) return rc;
+  if (tokens < 0 || !cu || !start || heads <= 0 || heads % c->kv_heads) return B200_ERR_ARG;
+  if (tokens == 0) return B200_OK;
+  if (!qkv || !q_out || (cos == nullptr) != (sin == nullptr)) return B200_ERR_ARG;
+  if (cos && (rot <= 0 || rot % 16 || rot > c->head_dim || rope_rows <= 0)) return B200_ERR_TILE;
+  if (ld < static_cast<long long>(heads + 2 * c->kv_heads) * c->head_dim) return B200_ERR_ARG;
+  if (!al16(qkv) || !al16(q_out) || ld % 8) return B200_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  Kv8AppendParams p{};
+  p.c = cache8_of(c);
+  p.qkv = static_cast<const uint16_t*>(qkv);
+  p.ld = ld;
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.cu = cu;
+  p.start = start;
+  p.cos = cos;
+  p.sin = sin;
+  p.rot = cos ? rot : 0;
+  p.interleaved = interleaved;
+  p.rope_rows = rope_rows;
+  p.tokens = tokens;
+  p.batch = c->batch;
+  p.heads = heads;
+  const long long by_block = static_cast<long long>(tokens) / c->page_size + 2LL * c->batch;
+  if (by_block > 0x7fffffffLL) return B200_ERR_TILE;
+  p.by_token = tokens <= by_block;
+  const unsigned units = static_cast<unsigned>(p.by_token ? tokens : by_block);
+  const int smem = c->page_size * c->head_dim * 2;
+  launch_kernel(k_kv8_append, dim3(units, 3u * c->kv_heads), dim3(p.by_token ? 64 : 256), smem, st, p);
+  return launch_status();
+}
+
+int kv8_read_impl(const B200KvCache8* c, const int* cu, const int* start, const int* lens, void* k_out, void* v_out,
+                  int tokens, cudaStream_t st) {
+  if (int rc = cache8_check(c)) return rc;
+  if (tokens < 0 || !cu || !start || !lens) return B200_ERR_ARG;
+  if (tokens == 0) return B200_OK;
+  if (!k_out || !v_out) return B200_ERR_ARG;
+  if (!al16(k_out) || !al16(v_out)) return B200_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  Kv8ReadParams p{};
+  p.c = cache8_of(c);
+  p.cu = cu;
+  p.start = start;
+  p.lens = lens;
+  p.k_out = static_cast<uint16_t*>(k_out);
+  p.v_out = static_cast<uint16_t*>(v_out);
+  p.tokens = tokens;
+  p.batch = c->batch;
+  const int per = 256 / (c->head_dim / 8);
+  launch_kernel(k_kv8_read, dim3((tokens + per - 1) / per, c->kv_heads), dim3(256), 0, st, p);
+  return launch_status();
+}
+
+// Rows of a tile: one column tile of 8 where a key head's rows fit it, else two.
+int attn8_rows(int max_q_len, int group) { return static_cast<long long>(max_q_len) * group <= 8 ? 8 : 16; }
+// CTAs of 8 warps an SM holds (shared memory; head_dim 128 takes all of it)
+int attn8_ctas(int head_dim) { return (head_dim == 128 ? 1 : 2) * num_sms(); }
+
+size_t attn8_workspace(int batch, int heads, int kv_heads, int head_dim, int max_q_len) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_q_len <= 0) return 0;
+  const size_t slots = static_cast<size_t>(attn8_ctas(head_dim)) * ATTN8_WARPS * 2 * attn8_rows(max_q_len, heads / kv_heads);
+  return slots * (head_dim + 2) * sizeof(float) + (static_cast<size_t>(batch) + 1) * sizeof(int);
+}
+
+template <int D, int NT>
+int launch_attn8(Attn8Params& p, int ctas, long long rows, cudaStream_t st) {
+  using C = Attn8Cfg<D, NT>;
+  p.warps = ctas * ATTN8_WARPS;
+  p.plan = reinterpret_cast<int*>(p.part + static_cast<size_t>(p.warps) * 2 * C::ROWS * (D + 2));
+  // whole row tiles keep every warp busy when there are several a warp; else the keys are cut too
+  p.split = rows / C::ROWS * p.c.kv_heads < 4LL * p.warps;
+  auto kern = k_attn8<D, NT>;
+  const int smem = C::SMEM + (ATTN8_MAX_BATCH + 1) * 4;
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
+  launch_kernel(kern, dim3(ctas), dim3(32 * ATTN8_WARPS), C::SMEM + (p.batch + 1) * 4, st, p);
+  if (int rc = launch_status()) return rc;
+  if (p.split) {
+    launch_kernel(k_attn8_join<D, NT>, dim3(static_cast<unsigned>(rows / C::ROWS + p.batch), p.c.kv_heads), dim3(128), 0,
+                  st, p);
+    return launch_status();
+  }
+  return B200_OK;
+}
+
+int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, long long ld_out, const int* cu,
+               const int* lens, int tokens, int heads, int max_q_len, float scale, void* ws, size_t ws_bytes,
+               cudaStream_t st) {
+  if (int rc = cache8_check(c)) return rc;
+  if (tokens < 0 || !cu || !lens || heads <= 0 || heads % c->kv_heads || max_q_len < 0) return B200_ERR_ARG;
+  if (tokens == 0) return B200_OK;
+  if (!q || !out || max_q_len == 0) return B200_ERR_ARG;
+  const long long width = static_cast<long long>(heads) * c->head_dim;
+  if (ld_q < width || ld_out < width) return B200_ERR_ARG;
+  if (!al16(q) || !al16(out) || ld_q % 8 || ld_out % 8) return B200_ERR_ALIGN;
+  const int group = heads / c->kv_heads;
+  const long long rows = static_cast<long long>(tokens) * group;
+  // the line of (sequence, head, row tile, chunk) work is numbered in 32 bits
+  const long long chunks = static_cast<long long>(c->table_width) * c->page_size / ATTN8_CHUNK + 2;
+  if (rows > 0x7fffffffLL || (rows / 8 + c->batch) * c->kv_heads * chunks > 0x7fffffffLL) return B200_ERR_TILE;
+  if (!ws || ws_bytes < attn8_workspace(c->batch, heads, c->kv_heads, c->head_dim, max_q_len)) return B200_ERR_WORKSPACE;
+  if (!al16(ws)) return B200_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  Attn8Params p{};
+  p.c = cache8_of(c);
+  p.q = static_cast<const uint16_t*>(q);
+  p.out = static_cast<uint16_t*>(out);
+  p.ld_q = ld_q;
+  p.ld_out = ld_out;
+  p.cu = cu;
+  p.lens = lens;
+  p.tokens = tokens;
+  p.batch = c->batch;
+  p.heads = heads;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part = static_cast<float*>(ws);
+  const int ctas = attn8_ctas(c->head_dim);
+  const bool one = attn8_rows(max_q_len, group) == 8;
+  switch (c->head_dim) {
+    case 32: return one ? launch_attn8<32, 1>(p, ctas, rows, st) : launch_attn8<32, 2>(p, ctas, rows, st);
+    case 64: return one ? launch_attn8<64, 1>(p, ctas, rows, st) : launch_attn8<64, 2>(p, ctas, rows, st);
+    default: return one ? launch_attn8<128, 1>(p, ctas, rows, st) : launch_attn8<128, 2>(p, ctas, rows, st);
+  }
+}
+
+// 8-bit [rows, cols] matrix with row pitch ld bytes: boxes of 128 bytes x box_rows, SWIZZLE_128B
+int make_map_i8(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+  return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, cols, ld, 128, box_rows,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+long long i8_pitch(int K) { return (static_cast<long long>(K) + 15) / 16 * 16; }
+
+size_t linear_i8_workspace(int M, int K) {
+  if (M <= 0 || K <= 0) return 0;
+  return static_cast<size_t>(M) * i8_pitch(K) + static_cast<size_t>(M) * sizeof(float);
+}
+
+int quantize_rows_impl(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scale, int m,
+                       int k, cudaStream_t st) {
+  if (x_type < 0 || x_type > 2) return B200_ERR_CONFIG;
+  if (m < 0 || k <= 0 || ld_x < k || ld_codes < k) return B200_ERR_ARG;
+  if (m == 0) return B200_OK;
+  if (!x || !codes || !scale) return B200_ERR_ARG;
+  if (int rc = check_arch()) return rc;
+  auto kern = x_type == DT_F16 ? k_quant_rows<DT_F16> : x_type == DT_BF16 ? k_quant_rows<DT_BF16> : k_quant_rows<DT_F32>;
+  launch_kernel(kern, dim3(m), dim3(256), 0, st, x, ld_x, static_cast<int8_t*>(codes), ld_codes, scale, m, k);
+  return launch_status();
+}
+
+int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
+  if (!a || a->m < 0 || a->n <= 0 || a->k <= 0) return B200_ERR_ARG;
+  if (a->x_type < 0 || a->x_type > 2 || a->out_type < 0 || a->out_type > 2) return B200_ERR_CONFIG;
+  if (a->resid && (a->out_type != DT_F32 || a->gelu)) return B200_ERR_CONFIG;
+  if (a->m == 0) return B200_OK;
+  if (!a->x || !a->w || !a->w_scale || !a->out) return B200_ERR_ARG;
+  if (a->ld_x < a->k || a->ld_w < a->k || a->ld_out < a->n || (a->resid && a->ld_resid < a->n)) return B200_ERR_ARG;
+  if (a->ld_w % 16 || !al16(a->w)) return B200_ERR_ALIGN;
+  // rounding x's sums in int32: |sum| <= 127 * 127 * k
+  if (a->k > 133000) return B200_ERR_TILE;
+  if (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k)) return B200_ERR_WORKSPACE;
+  if (!al16(a->workspace)) return B200_ERR_ALIGN;
+  if (int rc = check_arch()) return rc;
+  const long long pitch = i8_pitch(a->k);
+  int8_t* codes = static_cast<int8_t*>(a->workspace);
+  float* sx = reinterpret_cast<float*>(codes + static_cast<size_t>(a->m) * pitch);
+  if (int rc = quantize_rows_impl(a->x, a->x_type, a->ld_x, codes, pitch, sx, a->m, a->k, st)) return rc;
+  constexpr int BN = 128, STAGES = 6;
+  CUtensorMap ta, tw;
+  if (int rc = make_map_i8(&ta, codes, a->m, a->k, pitch, 128)) return rc;
+  if (int rc = make_map_i8(&tw, a->w, a->n, a->k, a->ld_w, BN)) return rc;
+  GemmI8Params p{};
+  p.M = a->m;
+  p.N = a->n;
+  p.K = a->k;
+  p.sx = sx;
+  p.sw = a->w_scale;
+  p.bias = a->bias;
+  p.resid = a->resid;
+  p.ld_resid = a->ld_resid;
+  p.out = a->out;
+  p.ld_out = a->ld_out;
+  p.gelu = a->gelu;
+  p.dt = a->out_type;
+  auto kern = k_gemm_i8<BN, STAGES>;
+  const int smem = STAGES * (128 + BN) * 128 + 256 + 1024;
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
+  const long long tiles = static_cast<long long>((a->m + 127) / 128) * ((a->n + BN - 1) / BN);
+  if (tiles > 0x7fffffffLL) return B200_ERR_TILE;
+  launch_kernel(kern, dim3(static_cast<unsigned>(std::min<long long>(tiles, num_sms()))), dim3(GEMM_THREADS), smem, st,
+                ta, tw, p);
+  return launch_status();
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_kv8_append(const B200KvCache8* cache, const void* qkv, long long ld_qkv, void* q_out, const int* cu,
+                    const int* start, const float* cos, const float* sin, int rot, int interleaved, int rope_rows,
+                    int tokens, int heads, b200_stream_t stream) {
+  return kv8_append_impl(cache, qkv, ld_qkv, q_out, cu, start, cos, sin, rot, interleaved, rope_rows, tokens, heads,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int b200_kv8_read(const B200KvCache8* cache, const int* cu, const int* start, const int* lens, void* k_out, void* v_out,
+                  int tokens, b200_stream_t stream) {
+  return kv8_read_impl(cache, cu, start, lens, k_out, v_out, tokens, static_cast<cudaStream_t>(stream));
+}
+
+size_t b200_kv8_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int max_q_len) {
+  return attn8_workspace(batch, heads, kv_heads, head_dim, max_q_len);
+}
+
+int b200_kv8_attention(const B200KvCache8* cache, const void* q, long long ld_q, void* out, long long ld_out,
+                       const int* cu, const int* lens, int tokens, int heads, int max_q_len, float scale,
+                       void* workspace, size_t workspace_bytes, b200_stream_t stream) {
+  return attn8_impl(cache, q, ld_q, out, ld_out, cu, lens, tokens, heads, max_q_len, scale, workspace, workspace_bytes,
+                    static_cast<cudaStream_t>(stream));
+}
+
+int b200_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scale,
+                          int m, int k, b200_stream_t stream) {
+  return quantize_rows_impl(x, x_type, ld_x, codes, ld_codes, scale, m, k, static_cast<cudaStream_t>(stream));
+}
+
+size_t b200_linear_i8_workspace_bytes(int m, int k) { return linear_i8_workspace(m, k); }
+
+int b200_linear_i8(const B200LinearI8Args* args, b200_stream_t stream) {
+  return linear_i8_impl(args, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

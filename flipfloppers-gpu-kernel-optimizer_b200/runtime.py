@@ -99,6 +99,26 @@ class FusedSmallArgs(ctypes.Structure):
     ]
 
 
+class KvCache8(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", _vp), ("v_pages", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_newest", _vp), ("v_newest", _vp),
+        ("table", _vp), ("rows", _vp),
+        ("num_pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("page_size", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("newest_rows", ctypes.c_int), ("table_width", ctypes.c_int),
+        ("batch", ctypes.c_int), ("bf16", ctypes.c_int),
+    ]
+
+
+class LinearI8Args(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("w", _vp), ("w_scale", _vp), ("bias", _vp), ("resid", _vp), ("out", _vp),
+        ("ld_x", _c_ll), ("ld_w", _c_ll), ("ld_resid", _c_ll), ("ld_out", _c_ll),
+        ("m", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int),
+        ("x_type", ctypes.c_int), ("out_type", ctypes.c_int), ("gelu", ctypes.c_int),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # (name, restype, argtypes) of every exported symbol; include/b200_block.h is the source of truth.
 EXPORTS = [
     ("b200_abi_version", ctypes.c_int, []),
@@ -126,6 +146,18 @@ EXPORTS = [
     ("b200_block_fused_small_launch", ctypes.c_int, [ctypes.POINTER(FusedSmallArgs), _vp]),
     ("b200_block_chunked_workspace_bytes", ctypes.c_size_t, [_c_ll, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     ("b200_block_forward_chunked", ctypes.c_int, [ctypes.POINTER(BlockArgs), ctypes.c_int, _vp]),
+    ("b200_kv8_append", ctypes.c_int,
+     [ctypes.POINTER(KvCache8), _vp, _c_ll, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+      ctypes.c_int, ctypes.c_int, _vp]),
+    ("b200_kv8_read", ctypes.c_int, [ctypes.POINTER(KvCache8), _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _vp]),
+    ("b200_kv8_attention_workspace_bytes", ctypes.c_size_t, [ctypes.c_int] * 5),
+    ("b200_kv8_attention", ctypes.c_int,
+     [ctypes.POINTER(KvCache8), _vp, _c_ll, _vp, _c_ll, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+      ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    ("b200_quantize_rows_i8", ctypes.c_int,
+     [_vp, ctypes.c_int, _c_ll, _vp, _c_ll, _vp, ctypes.c_int, ctypes.c_int, _vp]),
+    ("b200_linear_i8_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),
+    ("b200_linear_i8", ctypes.c_int, [ctypes.POINTER(LinearI8Args), _vp]),
 ]
 
 

@@ -309,6 +309,91 @@ int b200_block_fused_small_launch(const B200FusedSmallArgs* args, b200_stream_t 
 #define B200_NOALLOC_SCRATCH_BYTES (32u * 1024u * 1024u)
 int b200_block_forward_noalloc(const B200BlockArgs* args, b200_stream_t stream);
 
+/* ------------------------------------------------------------------ 8-bit serving
+ * A paged key/value cache in 8 bits, for decoding token by token.  A page holds
+ * one block of page_size tokens of every key head:
+ *   k_pages uint8 [num_pages][kv_heads][page_size][head_dim]
+ *   v_pages uint8 [num_pages][kv_heads][page_size/4][head_dim][4]
+ *   k_scale, v_scale fp32 [num_pages][kv_heads]
+ * a code c standing for (c - 128) * scale.  The newest two blocks of a sequence
+ * are held in 16 bits as well:
+ *   k_newest [newest_rows][2][kv_heads][page_size][head_dim]
+ *   v_newest [newest_rows][2][kv_heads][page_size/4][head_dim][4]
+ * block j in slot j % 2, sequence b in row rows[b] (rows NULL: row b).  A block
+ * that is not full is read from there; when its last token arrives it is
+ * quantized from its 16-bit values (scale = largest magnitude / 127; a block with
+ * an infinity or NaN gets a NaN scale).  A sequence may be shortened by starting
+ * the next append earlier, down to the first token of its newest two blocks.
+ * table [batch][table_width]: the page of each block of each sequence.
+ * head_dim 32, 64 or 128; page_size 16, 32, 64 or 128; batch <= 4096.  All on the
+ * device, 16-byte aligned.  A page, row or length outside its buffer is skipped
+ * and sets the device error word (7). */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  float* k_scale;
+  float* v_scale;
+  void* k_newest;
+  void* v_newest;
+  const int* table;
+  const int* rows;
+  int num_pages, kv_heads, page_size, head_dim, newest_rows, table_width, batch;
+  int bf16; /* the 16-bit type: 0 fp16, 1 bf16 */
+} B200KvCache8;
+
+/* qkv [tokens, (heads + 2*kv_heads)*head_dim] (16 bits, row stride ld_qkv, a
+ * multiple of 8): row cu[b] + i is token start[b] + i of sequence b.  q and k are
+ * rotated by position (the first `rot` channels of a head, a multiple of 16; pairs
+ * (i, i + rot/2), or (2i, 2i+1) if interleaved; cos and sin fp32
+ * [rope_rows, rot/2]; cos NULL: no rotation), q goes to q_out
+ * [tokens, heads, head_dim], k and v to the cache.  cu [batch+1], start [batch]. */
+int b200_kv8_append(const B200KvCache8* cache, const void* qkv, long long ld_qkv, void* q_out, const int* cu,
+                    const int* start, const float* cos, const float* sin, int rot, int interleaved, int rope_rows,
+                    int tokens, int heads, b200_stream_t stream);
+
+/* The values attention sees, as 16-bit rows: row cu[b] + i of k_out and v_out
+ * [tokens, kv_heads, head_dim] is token start[b] + i of sequence b, of which
+ * lens[b] tokens are cached. */
+int b200_kv8_read(const B200KvCache8* cache, const int* cu, const int* start, const int* lens, void* k_out, void* v_out,
+                  int tokens, b200_stream_t stream);
+
+/* Attention of the newest tokens over the cache: row cu[b] + i of q
+ * [tokens, heads, head_dim] is the token at position lens[b] - n + i of sequence b
+ * (n = cu[b+1] - cu[b] new tokens, all appended already), which sees the keys up
+ * to its own; heads % kv_heads == 0, consecutive query heads share a key head.  A
+ * row with no key (position < 0) gives zeros.  max_q_len >= every n.  No atomics:
+ * the same inputs give the same bits. */
+size_t b200_kv8_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int max_q_len);
+int b200_kv8_attention(const B200KvCache8* cache, const void* q, long long ld_q, void* out, long long ld_out,
+                       const int* cu, const int* lens, int tokens, int heads, int max_q_len, float scale,
+                       void* workspace, size_t workspace_bytes, b200_stream_t stream);
+
+/* out[M,N] = epi( (round(x / sx) . w^T) * sx[row] * w_scale[col] + bias[col] ) with
+ * sx = the row's largest magnitude / 127 and exact integer sums.  x [m, k] of x_type,
+ * w int8 [n, k] with row pitch ld_w (a multiple of 16 bytes), bias fp32 or NULL, gelu
+ * != 0: exact GELU; resid (fp32 [m, n], out_type fp32, no GELU) is added last and may
+ * be out itself.  Types: 0 fp16, 1 bf16, 2 fp32.  Any m, n, k up to k = 133000.  A row
+ * with an infinity or NaN gives NaN. */
+typedef struct {
+  const void* x;
+  const void* w;
+  const float* w_scale;
+  const float* bias;
+  const float* resid;
+  void* out;
+  long long ld_x, ld_w, ld_resid, ld_out;
+  int m, n, k;
+  int x_type, out_type, gelu;
+  void* workspace;        /* >= b200_linear_i8_workspace_bytes(m, k), 16-byte aligned */
+  size_t workspace_bytes;
+} B200LinearI8Args;
+/* x [m, k] of x_type -> int8 codes [m, k] (row pitch ld_codes bytes) and scale [m]: the
+ * quantization b200_linear_i8 gives x, and what lays out a weight for it. */
+int b200_quantize_rows_i8(const void* x, int x_type, long long ld_x, void* codes, long long ld_codes, float* scale,
+                          int m, int k, b200_stream_t stream);
+size_t b200_linear_i8_workspace_bytes(int m, int k);
+int b200_linear_i8(const B200LinearI8Args* args, b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

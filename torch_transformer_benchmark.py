@@ -41,6 +41,7 @@ def load_package():
 _pkg = load_package()
 TransformerConfig = _pkg.TransformerConfig
 UserOptimizedTransformer = _pkg.UserOptimizedTransformer
+serving = _pkg.serving
 
 
 def main() -> int:
