@@ -5,51 +5,118 @@
 // bias + GELU (out in x's type or fp32), bias + fp32 residual.
 #pragma once
 
-#include "gemm.cuh"
+#include "gemm2.cuh"
 #include "kv8.cuh"
 
 namespace b200 {
 
 enum Dt : int { DT_F16 = 0, DT_BF16 = 1, DT_F32 = 2 };
 
-// x [M, K] (row stride ldx elements) -> codes int8 [M, ldq], scale [M].  A row with an
-// infinity or NaN gets a NaN scale, so its outputs are NaN.  One CTA a row; the row is
-// read twice, the second time from L1/L2.
+// 16 consecutive values of a row from k on (zeros past K); vec: all 16 exist and the address is 16-byte aligned
 template <int DT>
-__global__ void __launch_bounds__(256) k_quant_rows(const void* x, long long ldx, int8_t* q, long long ldq,
-                                                    float* scale, int M, int K) {
-  __shared__ unsigned tops[8];
-  griddep_sync();
-  const int tid = threadIdx.x;
-  const size_t row = blockIdx.x;
-  auto at = [&](int k) -> float {
-    if constexpr (DT == DT_F32) return static_cast<const float*>(x)[row * ldx + k];
-    else return h16_to_f(static_cast<const uint16_t*>(x)[row * ldx + k], DT == DT_BF16);
-  };
-  unsigned top = 0;
-  for (int k = tid; k < K; k += 256) top = max(top, __float_as_uint(at(k)) & 0x7fffffffu);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) tops[tid >> 5] = top;
-  __syncthreads();
-  for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
-  const float s = top < 0x7f800000u ? __fmul_rn(__uint_as_float(top), 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
-  if (tid == 0) scale[row] = s;
-  for (int k = tid; k < K; k += 256) {
-    const float r = s > 0.f ? rintf(__fdiv_rn(at(k), s)) : 0.f;
-    q[row * ldq + k] = static_cast<int8_t>(static_cast<int>(fminf(fmaxf(r, -127.f), 127.f)));
+__device__ __forceinline__ void load_row16(const void* x, size_t base, int k, int K, bool vec, float (&v)[16]) {
+  if (vec) {
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + base + k) + i);
+        v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float u[8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + base + k) + i), DT == DT_BF16, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * i + j] = u[j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (k + j >= K) v[j] = 0.f;
+      else if constexpr (DT == DT_F32) v[j] = __ldg(static_cast<const float*>(x) + base + k + j);
+      else v[j] = h16_to_f(__ldg(static_cast<const uint16_t*>(x) + base + k + j), DT == DT_BF16);
+    }
   }
 }
+
+// rint(x / s), x / s rounded to fp32 first, for |x| <= 127.5 s.  The product with the reciprocal is within 2^-20 of
+// the quotient's magnitude bound, so only quotients that near a half need the division itself.
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+  const float y = x * inv, r = rintf(y);
+  return fabsf(fabsf(y - r) - 0.5f) > 2e-3f ? r : rintf(__fdiv_rn(x, s));
+}
+__device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
+  return (static_cast<uint32_t>(static_cast<int>(a)) & 0xffu) | (static_cast<uint32_t>(static_cast<int>(b)) & 0xffu) << 8 |
+         (static_cast<uint32_t>(static_cast<int>(c)) & 0xffu) << 16 | static_cast<uint32_t>(static_cast<int>(d)) << 24;
+}
+
+// x [M, K] (row stride ldx elements) -> codes int8 [M, ldq], scale [M].  A row with an
+// infinity or NaN gets a NaN scale, so its outputs are NaN.  TPR threads a row (a warp
+// for rows up to 2048 values); the row is read twice, the second time from L1.
+// Memory-bound.  vec: x's rows start 16-byte aligned; ldq is a multiple of 16 or the
+// codes leave one by one.
+template <int DT, int TPR>
+__global__ void __launch_bounds__(256) k_quant_rows(const void* x, long long ldx, int8_t* q, long long ldq,
+                                                    float* scale, int M, int K, int vec) {
+  __shared__ unsigned tops[8];
+  griddep_sync();
+  const int tid = threadIdx.x % TPR;
+  const size_t row = static_cast<size_t>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  if (TPR == 32 && row >= static_cast<size_t>(M)) return;
+  const size_t base = row * ldx;
+  unsigned top = 0;
+  for (int k = tid * 16; k < K; k += TPR * 16) {
+    float v[16];
+    load_row16<DT>(x, base, k, K, vec && k + 16 <= K, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (TPR > 32) {
+    if ((tid & 31) == 0) tops[tid >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < TPR / 32; ++i) top = max(top, tops[i]);
+  }
+  const float s = top < 0x7f800000u ? __fmul_rn(__uint_as_float(top), 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+  if (tid == 0) scale[row] = s;
+  const bool live = s > 0.f;                // false: a row of zeros, or NaN
+  const bool small = s < 1e-30f;            // 1 / s could overflow: divide
+  const float inv = __fdiv_rn(1.f, s);
+  for (int k = tid * 16; k < K; k += TPR * 16) {
+    float v[16];
+    load_row16<DT>(x, base, k, K, vec && k + 16 <= K, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float r = !live ? 0.f : small ? rintf(__fdiv_rn(v[j], s)) : quotient(v[j], s, inv);
+      v[j] = fminf(fmaxf(r, -127.f), 127.f);
+    }
+    uint4 w = make_uint4(pack_codes(v[0], v[1], v[2], v[3]), pack_codes(v[4], v[5], v[6], v[7]),
+                         pack_codes(v[8], v[9], v[10], v[11]), pack_codes(v[12], v[13], v[14], v[15]));
+    int8_t* to = q + row * ldq + k;
+    if (k + 16 <= ldq && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      *reinterpret_cast<uint4*>(to) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (k + j < K) to[j] = static_cast<int8_t>(v[j]);
+    }
+  }
+}
+
+enum I8Epilogue : int { I8_BIAS = 0, I8_GELU = 1, I8_RESID = 2 };
 
 struct GemmI8Params {
   int M, N, K;
   const float* sx;     // [M]
   const float* sw;     // [N]
   const float* bias;   // [N], may be null
-  const float* resid;  // fp32 [M, N], row stride ld_resid, may be null
+  const float* resid;  // I8_RESID: fp32 [M, N], row stride ld_resid
   long long ld_resid;
   void* out;           // [M, N], row stride ld_out
   long long ld_out;
-  int gelu, dt;        // output type
+  int tma_out;         // out's rows are 16-byte aligned: tiles leave by TMA store
 };
 
 // kind::i8 instruction descriptor: int32 accumulators (bits 4-5 = 2), signed 8-bit A and B, both K-major
@@ -66,37 +133,121 @@ __device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t adesc, uint
       : "memory");
 }
 
-// One row's `cols` (up to 32) results from column col0 on: v holds the int32 sums.
-__device__ __forceinline__ void gemm_i8_row(const GemmI8Params& p, int row, int col0, float (&v)[32]) {
-  const int cols = min(32, p.N - col0);
-  if (row >= p.M || cols <= 0) return;
-  const float sx = __ldg(p.sx + row);
+template <int DT>
+struct I8Out {
+  static constexpr int CC = DT == DT_F32 ? 16 : 32;  // columns of a 64-byte chunk row
+};
+constexpr int I8_STG_WARP = 4096 + 1024;  // per epilogue warp: two 2 KB chunk slots, then 128 columns' scales and biases
+
+// Scales and biases of the 128 columns from col0 on into the warp's own shared memory (0 past N).
+__device__ __forceinline__ void i8_columns(const GemmI8Params& p, int col0, float* cols, int lane) {
+  __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const int c = min(col0 + j, p.N - 1);
-    float y = __fmul_rn(__fmul_rn(static_cast<float>(__float_as_int(v[j])), sx), __ldg(p.sw + c));
-    if (p.bias) y = __fadd_rn(y, __ldg(p.bias + c));
-    if (p.gelu) y = gelu_as(y);
-    if (p.resid) y += __ldg(p.resid + row * p.ld_resid + c);
-    v[j] = y;
+  for (int i = 0; i < 4; ++i) {
+    const int c = col0 + lane + 32 * i;
+    cols[lane + 32 * i] = c < p.N ? __ldg(p.sw + c) : 0.f;
+    cols[128 + lane + 32 * i] = p.bias != nullptr && c < p.N ? __ldg(p.bias + c) : 0.f;
   }
-  if (p.dt == DT_F32) {
-    float* o = static_cast<float*>(p.out) + row * p.ld_out + col0;
-    for (int j = 0; j < cols; ++j) o[j] = v[j];
-  } else {
-    uint16_t* o = static_cast<uint16_t*>(p.out) + row * p.ld_out + col0;
-    for (int j = 0; j < cols; ++j) o[j] = static_cast<uint16_t>(f_to_h16(v[j], p.dt == DT_BF16));
+  __syncwarp();
+}
+
+// Epilogue of `width` (<= 128) columns of an accumulator tile for one warp: 32 rows from row0, one a lane.
+// Chunks of 64 bytes a row are staged (SWIZZLE_64B) in the warp's two slots and leave by TMA store, or, where
+// out's rows are not 16-byte aligned, element by element along the rows.
+template <int DT, int EPI>
+__device__ __forceinline__ void i8_epilogue(const CUtensorMap* tmO, const GemmI8Params& p, uint32_t taddr, int width,
+                                            int col0, int row0, uint8_t* stg, int& gc, int lane) {
+  constexpr int CC = I8Out<DT>::CC;
+  const float* cols = reinterpret_cast<const float*>(stg + 4096);
+  const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
+  const int row = row0 + lane;
+  const float sx = row < p.M ? __ldg(p.sx + row) : 0.f;
+  const uint64_t sx2 = f2pk(sx, sx);
+#pragma unroll 1
+  for (int c = 0; c < width; c += CC, ++gc) {
+    const int col = col0 + c;
+    if (col >= p.N) break;
+    float v[CC];
+    if constexpr (DT == DT_F32) tmem_ld16(taddr + c, v);
+    else tmem_ld32(taddr + c, v);
+    if constexpr (EPI == I8_RESID) {
+      if (row < p.M) {
+        const float* r = p.resid + row * p.ld_resid + col;
+        float u[CC];
+#pragma unroll
+        for (int j = 0; j < CC; ++j) u[j] = col + j < p.N ? __ldg(r + j) : 0.f;
+#pragma unroll
+        for (int j = 0; j < CC; ++j)
+          v[j] = __fadd_rn(u[j], __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(v[j])), sx), cols[c + j]),
+                                           cols[128 + c + j]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CC; j += 2) {
+        uint64_t y = f2pk(__int2float_rn(__float_as_int(v[j])), __int2float_rn(__float_as_int(v[j + 1])));
+        y = f2mul(f2mul(y, sx2), *reinterpret_cast<const uint64_t*>(cols + c + j));
+        y = f2add(y, *reinterpret_cast<const uint64_t*>(cols + 128 + c + j));
+        f2upk(y, v[j], v[j + 1]);
+        if constexpr (EPI == I8_GELU) gelu_as2(v[j], v[j + 1]);
+      }
+    }
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if constexpr (DT == DT_F32) w[j] = __float_as_uint(v[j]);
+      else if constexpr (DT == DT_F16) w[j] = pack_half2(v[2 * j], v[2 * j + 1]);
+      else w[j] = f_to_h16(v[2 * j], 1) | f_to_h16(v[2 * j + 1], 1) << 16;
+    }
+    uint8_t* slot = stg + (gc & 1) * 2048;
+    if (lane == 0) bulk_wait_read_1();  // the slot's previous chunk has left
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4*>(slot + lane * 64 + ((j ^ sw) << 4)) =
+          make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    if (p.tma_out) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tmO, slot, col, row0);
+        bulk_commit();
+      }
+    } else {
+      __syncwarp();
+      const int rows = min(32, p.M - row0);
+      if constexpr (DT == DT_F32) {
+        for (int r = lane >> 4; r < rows; r += 2) {
+          const int j = lane & 15;
+          if (col + j < p.N)
+            static_cast<float*>(p.out)[(row0 + r) * p.ld_out + col + j] = *reinterpret_cast<const float*>(
+                slot + r * 64 + (((j >> 2) ^ ((r >> 1) & 3)) << 4) + (j & 3) * 4);
+        }
+      } else {
+        for (int r = 0; r < rows; ++r)
+          if (col + lane < p.N)
+            static_cast<uint16_t*>(p.out)[(row0 + r) * p.ld_out + col + lane] = *reinterpret_cast<const uint16_t*>(
+                slot + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+      }
+    }
   }
 }
 
 // The persistent schedule of k_gemm_tn with 128-byte K slices of 8-bit operands.
 template <int BN, int STAGES>
+struct GemmI8Smem {
+  static constexpr int A_BYTES = 128 * 128, STAGE_BYTES = A_BYTES + BN * 128;
+  static constexpr int STG_OFF = STAGES * STAGE_BYTES, BAR_OFF = STG_OFF + 8 * I8_STG_WARP;
+  static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+};
+template <int BN, int STAGES, int DT, int EPI>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
-    k_gemm_i8(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const GemmI8Params p) {
-  constexpr int A_BYTES = 128 * 128, STAGE_BYTES = A_BYTES + BN * 128;
+    k_gemm_i8(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+              const __grid_constant__ CUtensorMap tmO, const GemmI8Params p) {
+  using L = GemmI8Smem<BN, STAGES>;
+  constexpr int A_BYTES = L::A_BYTES, STAGE_BYTES = L::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align1024(smem_raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
@@ -191,22 +342,22 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* stg = smem + L::STG_OFF + (warp - 2) * I8_STG_WARP;
+    int gc = 0;
     for (int i = 0; i < my_tiles; ++i) {
       const int b = i & 1;
       const int t = static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x);
-      const int row = (t / ntl) * 128 + q * 32 + lane, n0 = (t % ntl) * BN;
+      const int row0 = (t / ntl) * 128 + q * 32, col0 = (t % ntl) * BN + half * (BN / 2);
+      i8_columns(p, col0, reinterpret_cast<float*>(stg + 4096), lane);
       const bool ok = mbar_wait_warp(&acc_full[b], (i >> 1) & 1, abort_flag, DERR_WAIT_MMA);
       if (!ok || *abort_flag) break;
       tc_fence_after();
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        float v[32];
-        tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BN + c, v);
-        gemm_i8_row(p, row, n0 + c, v);
-        __syncwarp();
-      }
+      i8_epilogue<DT, EPI>(&tmO, p, tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BN + half * (BN / 2), BN / 2, col0,
+                           row0, stg, gc, lane);
       tc_fence_before();
       mbar_arrive(&acc_empty[b]);
     }
+    if (lane == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncwarp();
@@ -214,6 +365,160 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// The same on CTA pairs, after k_gemm2_tn: one 256x256 tile a pair, each CTA staging its 128 rows of x's codes and
+// 128 rows of w per 128-byte K slice.
+constexpr int GEMM2_I8_STAGES = 5;
+constexpr int GEMM2_I8_EW = 8;
+struct Gemm2I8Smem {
+  static constexpr int A_BYTES = 128 * 128, STAGE_BYTES = 2 * A_BYTES;
+  static constexpr int STG_OFF = GEMM2_I8_STAGES * STAGE_BYTES, BAR_OFF = STG_OFF + GEMM2_I8_EW * I8_STG_WARP;
+  static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+};
+__device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}\n"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u),
+        "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+template <int DT, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * GEMM2_I8_EW, 1)
+    k_gemm2_i8(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+               const __grid_constant__ CUtensorMap tmO, const GemmI8Params p) {
+  constexpr int STAGES = GEMM2_I8_STAGES, EW = GEMM2_I8_EW;
+  using L = Gemm2I8Smem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_align1024(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int cid = static_cast<int>(blockIdx.x) >> 1, ncl = static_cast<int>(gridDim.x) >> 1;
+  const int ntl = (p.N + 255) / 256, ntiles = (p.M + 255) / 256 * ntl;
+  const int my_tiles = (ntiles - cid + ncl - 1) / ncl;
+  const int nk = (p.K + 127) / 128;
+  constexpr uint32_t TMEM_COLS = 512;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * EW);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_sync();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmW);
+      int it = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const int t = cid + i * ncl;
+        const int m0 = (t / ntl) * 256, n0 = (t % ntl) * 256;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, abort_flag, DERR_WAIT_SLOT)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * L::STAGE_BYTES;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE_BYTES);
+          const uint32_t fbar = mapa_shared(smem_u32(&full[s]), 0);
+          tma_load_2d_pair(st, &tmA, fbar, kb * 128, m0 + 128 * static_cast<int>(rank));
+          tma_load_2d_pair(st + L::A_BYTES, &tmW, fbar, kb * 128, n0 + 128 * static_cast<int>(rank));
+        }
+      }
+      if (*abort_flag && rank == 0)
+        for (int j = (it > STAGES ? it - STAGES : 0); j < it; ++j) mbar_wait_drain(&full[j % STAGES], (j / STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc_i8(256, 256);
+      int it = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const int b = i & 1;
+        if (i >= 2 && !mbar_wait(&acc_empty[b], ((i >> 1) - 1) & 1, abort_flag, DERR_WAIT_MMA)) break;
+        tc_fence_after();
+        const uint32_t dcol = tmem + b * 256;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&full[s], (it / STAGES) & 1, abort_flag, DERR_WAIT_TMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + s * L::STAGE_BYTES), b_addr = a_addr + L::A_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_i8_ss_pair(dcol, make_sdesc(a_addr + kk * 32, 16, 1024, UMMA_SW128),
+                            make_sdesc(b_addr + kk * 32, 16, 1024, UMMA_SW128), idesc, (kb | kk) != 0 ? 1u : 0u);
+          tc_commit_pair(&empty[s], 0x3);
+        }
+        if (!ok) break;
+        tc_commit_pair(&acc_full[b], 0x3);
+      }
+      if (*abort_flag) {
+        tc_commit_pair(drain, 0x1);
+        mbar_wait_drain(drain, 0);
+      }
+    }
+  } else {
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    uint8_t* stg = smem + L::STG_OFF + (warp - 2) * I8_STG_WARP;
+    const uint32_t empty_leader0 = mapa_shared(smem_u32(&acc_empty[0]), 0);
+    int gc = 0;
+    for (int i = 0; i < my_tiles; ++i) {
+      const int b = i & 1;
+      const int t = cid + i * ncl;
+      const int row0 = (t / ntl) * 256 + 128 * static_cast<int>(rank) + q * 32, col0 = (t % ntl) * 256 + part * 128;
+      i8_columns(p, col0, reinterpret_cast<float*>(stg + 4096), lane);
+      const bool ok = mbar_wait_warp(&acc_full[b], (i >> 1) & 1, abort_flag, DERR_WAIT_MMA);
+      if (!ok || *abort_flag) break;
+      tc_fence_after();
+      i8_epilogue<DT, EPI>(&tmO, p, tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + part * 128, 128, col0, row0,
+                           stg, gc, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(empty_leader0 + b * 8);
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, TMEM_COLS);
   }
 }
 

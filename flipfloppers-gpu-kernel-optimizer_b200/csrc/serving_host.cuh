@@ -189,8 +189,47 @@ int quantize_rows_impl(const void* x, int x_type, long long ld_x, void* codes, l
   if (m == 0) return B200_OK;
   if (!x || !codes || !scale) return B200_ERR_ARG;
   if (int rc = check_arch()) return rc;
-  auto kern = x_type == DT_F16 ? k_quant_rows<DT_F16> : x_type == DT_BF16 ? k_quant_rows<DT_BF16> : k_quant_rows<DT_F32>;
-  launch_kernel(kern, dim3(m), dim3(256), 0, st, x, ld_x, static_cast<int8_t*>(codes), ld_codes, scale, m, k);
+  const int vec = al16(x) && ld_x % (x_type == DT_F32 ? 4 : 8) == 0;
+  auto run = [&](auto kern, int rows) {
+    launch_kernel(kern, dim3((m + rows - 1) / rows), dim3(256), 0, st, x, ld_x, static_cast<int8_t*>(codes), ld_codes, scale,
+                  m, k, vec);
+    return launch_status();
+  };
+  if (k <= 2048) {
+    if (x_type == DT_F16) return run(k_quant_rows<DT_F16, 32>, 8);
+    if (x_type == DT_BF16) return run(k_quant_rows<DT_BF16, 32>, 8);
+    return run(k_quant_rows<DT_F32, 32>, 8);
+  }
+  if (x_type == DT_F16) return run(k_quant_rows<DT_F16, 256>, 1);
+  if (x_type == DT_BF16) return run(k_quant_rows<DT_BF16, 256>, 1);
+  return run(k_quant_rows<DT_F32, 256>, 1);
+}
+
+template <int DT, int EPI>
+int launch_gemm_i8(const GemmI8Params& p, const CUtensorMap& ta, const void* w, long long ld_w, cudaStream_t st) {
+  CUtensorMap tw, to{};
+  if (p.tma_out)
+    if (int rc = make_map_2d(&to, DT == DT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                             DT == DT_F32 ? 4 : 2, p.out, p.M, p.N, p.ld_out, I8Out<DT>::CC, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+      return rc;
+  if (int rc = make_map_i8(&tw, w, p.N, p.K, ld_w, 128)) return rc;
+  if (p.M >= 512 && p.N >= 256) {
+    auto kern = k_gemm2_i8<DT, EPI>;
+    if (int rc = set_smem(reinterpret_cast<const void*>(kern), Gemm2I8Smem::TOTAL)) return rc;
+    const long long tiles = static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256);
+    if (tiles > 0x3fffffffLL) return B200_ERR_TILE;
+    launch_kernel(kern, dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, num_sms() / 2))),
+                  dim3(64 + 32 * GEMM2_I8_EW), Gemm2I8Smem::TOTAL, st, ta, tw, to, p);
+    return launch_status();
+  }
+  constexpr int BN = 128, STAGES = 5;
+  using L = GemmI8Smem<BN, STAGES>;
+  auto kern = k_gemm_i8<BN, STAGES, DT, EPI>;
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), L::TOTAL)) return rc;
+  const long long tiles = static_cast<long long>((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
+  if (tiles > 0x3fffffffLL) return B200_ERR_TILE;
+  launch_kernel(kern, dim3(static_cast<unsigned>(std::min<long long>(tiles, num_sms()))), dim3(GEMM_THREADS), L::TOTAL, st,
+                ta, tw, to, p);
   return launch_status();
 }
 
@@ -202,7 +241,7 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   if (!a->x || !a->w || !a->w_scale || !a->out) return B200_ERR_ARG;
   if (a->ld_x < a->k || a->ld_w < a->k || a->ld_out < a->n || (a->resid && a->ld_resid < a->n)) return B200_ERR_ARG;
   if (a->ld_w % 16 || !al16(a->w)) return B200_ERR_ALIGN;
-  // rounding x's sums in int32: |sum| <= 127 * 127 * k
+  // the sums are int32: |sum| <= 127 * 127 * k
   if (a->k > 133000) return B200_ERR_TILE;
   if (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k)) return B200_ERR_WORKSPACE;
   if (!al16(a->workspace)) return B200_ERR_ALIGN;
@@ -211,10 +250,8 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   int8_t* codes = static_cast<int8_t*>(a->workspace);
   float* sx = reinterpret_cast<float*>(codes + static_cast<size_t>(a->m) * pitch);
   if (int rc = quantize_rows_impl(a->x, a->x_type, a->ld_x, codes, pitch, sx, a->m, a->k, st)) return rc;
-  constexpr int BN = 128, STAGES = 6;
-  CUtensorMap ta, tw;
+  CUtensorMap ta;
   if (int rc = make_map_i8(&ta, codes, a->m, a->k, pitch, 128)) return rc;
-  if (int rc = make_map_i8(&tw, a->w, a->n, a->k, a->ld_w, BN)) return rc;
   GemmI8Params p{};
   p.M = a->m;
   p.N = a->n;
@@ -226,16 +263,12 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   p.ld_resid = a->ld_resid;
   p.out = a->out;
   p.ld_out = a->ld_out;
-  p.gelu = a->gelu;
-  p.dt = a->out_type;
-  auto kern = k_gemm_i8<BN, STAGES>;
-  const int smem = STAGES * (128 + BN) * 128 + 256 + 1024;
-  if (int rc = set_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
-  const long long tiles = static_cast<long long>((a->m + 127) / 128) * ((a->n + BN - 1) / BN);
-  if (tiles > 0x7fffffffLL) return B200_ERR_TILE;
-  launch_kernel(kern, dim3(static_cast<unsigned>(std::min<long long>(tiles, num_sms()))), dim3(GEMM_THREADS), smem, st,
-                ta, tw, p);
-  return launch_status();
+  p.tma_out = al16(a->out) && a->ld_out * (a->out_type == DT_F32 ? 4 : 2) % 16 == 0;
+  auto go = [&](auto f) { return f(p, ta, a->w, a->ld_w, st); };
+  if (a->resid) return go(launch_gemm_i8<DT_F32, I8_RESID>);
+  if (a->out_type == DT_F32) return a->gelu ? go(launch_gemm_i8<DT_F32, I8_GELU>) : go(launch_gemm_i8<DT_F32, I8_BIAS>);
+  if (a->out_type == DT_BF16) return a->gelu ? go(launch_gemm_i8<DT_BF16, I8_GELU>) : go(launch_gemm_i8<DT_BF16, I8_BIAS>);
+  return a->gelu ? go(launch_gemm_i8<DT_F16, I8_GELU>) : go(launch_gemm_i8<DT_F16, I8_BIAS>);
 }
 
 }  // namespace
