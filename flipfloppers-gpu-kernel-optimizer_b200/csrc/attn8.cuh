@@ -9,9 +9,10 @@
 //     pieces, one a warp, so ragged lengths load every SM alike; a piece that
 //     holds only part of a row tile leaves (max, sum, accumulator) in the
 //     workspace and k_attn8_join adds the parts in a fixed order;
-//   - codes go from HBM to shared memory by cp.async into slots private to the
-//     lane that will use them (ATTN8_STAGES chunks ahead), so only the lane's own
-//     wait_group orders them;
+//   - a chunk's K and V are 32 D contiguous bytes each: bulk copies bring them to the
+//     warp's own ring of shared memory, Attn8Cfg::STAGES chunks ahead (cp.async of 16
+//     bytes a lane asked L2 for every 32-byte sector twice and stopped at 3.2 TB/s;
+//     loads to registers kept too little in flight, 3.9 TB/s);
 //   - the products run as S^T = K Q^T and O^T = V^T P^T on m16n8k16 tensor-core
 //     steps: tokens (channels of V) fill the 16 rows, query rows the 8 columns, so
 //     up to 8 rows cost one column tile (NT = 1) and up to 16 two (NT = 2), and the
@@ -27,10 +28,8 @@
 
 namespace b200 {
 
-constexpr int ATTN8_WARPS = 8;
 constexpr int ATTN8_CHUNK = 32;   // tokens
-constexpr int ATTN8_STAGES = 3;
-constexpr int ATTN8_MAX_BATCH = 4096;
+constexpr int ATTN8_MAX_BATCH = 2048;
 
 struct Attn8Params {
   Kv8Cache c;
@@ -43,23 +42,29 @@ struct Attn8Params {
   int split;             // 1: cut the line of chunks into equal pieces; 0: whole row tiles
   float scale_log2;      // scale * log2(e)
   int warps;             // warps of the launch
-  int* plan;             // [batch + 1] first chunk of each sequence on the line (written by CTA 0)
+  int* plan;             // [batch + 1] first unit of each sequence on the line (written by CTA 0)
   float* part;           // [warps][2][rows][D] accumulators, then [warps][2][rows][2] (max, sum)
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same from zero
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 // a bf16 pair with its infinities and NaN taken as 0
@@ -67,19 +72,6 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t x) {
   if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
   if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
   return x;
-}
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
-  const int n = live ? BYTES : 0;  // 0: the slot is filled with zeros and src is not read
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 // Four codes -> two fp16 pairs of c - 128, exact: 0x6400 | c is 1024 + c.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -94,14 +86,14 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
 template <int D, int NT>
 struct Attn8Cfg {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int CB = D >= 64 ? 16 : 8;        // bytes a lane copies of a K row at once
-  static constexpr int NCH = D / (4 * CB);           // such copies a row
-  static constexpr int K_BYTES = ATTN8_CHUNK * D;    // one chunk
-  static constexpr int V_BYTES = ATTN8_CHUNK * D;
-  static constexpr int S_BYTES = 4 * 32 * 4;         // the chunk's scales, a copy a lane: K and V, two half chunks
-  static constexpr int STAGE = K_BYTES + V_BYTES + S_BYTES;
-  static constexpr int RING = ATTN8_STAGES * STAGE;  // one warp's
-  static constexpr int SMEM = ATTN8_WARPS * RING;
+  // Warps of the SM's one CTA, and chunks in each warp's ring of shared memory: about 200 KB in flight an SM
+  static constexpr int WARPS = D == 128 ? (NT == 1 ? 12 : 8) : NT == 1 ? 16 : 12;
+  static constexpr int STAGES = D == 128 ? (NT == 1 ? 2 : 3) : D == 64 ? (NT == 1 ? 3 : 4) : 6;
+  static constexpr int CB = D >= 64 ? 16 : 8;        // bytes a lane reads of a K row at once
+  static constexpr int NCH = D / (4 * CB);           // such reads a row
+  static constexpr int K_BYTES = ATTN8_CHUNK * D, STAGE = 2 * K_BYTES;  // K, then V of one chunk
+  static constexpr int RING = STAGES * STAGE;        // one warp's
+  static constexpr int BAR_OFF = WARPS * RING, TOTAL = BAR_OFF + WARPS * STAGES * 8 + 16;
 };
 
 // What one warp knows of the row tile it works on.
@@ -111,19 +103,37 @@ struct Attn8Seg {
   int q_len, t0;
 };
 
-// chunks of a sequence: those of the full blocks, then those of the newest block
+// chunks of a sequence: 32 tokens each of the full blocks, then 16 each of the newest block (as many bytes)
+__device__ __forceinline__ int attn8_full_chunks(int full_tokens) { return (full_tokens + ATTN8_CHUNK - 1) / ATTN8_CHUNK; }
 __device__ __forceinline__ int attn8_chunks(int len, int page) {
   const int full = len / page * page;
-  return max(1, (full + ATTN8_CHUNK - 1) / ATTN8_CHUNK + (len - full + ATTN8_CHUNK - 1) / ATTN8_CHUNK);
+  return attn8_full_chunks(full) + (len - full + 15) / 16;
+}
+// The line's units: a chunk of full blocks is one, a chunk of the newest block two and the start of a row tile two
+// (measured: its rows, pages and first copies take as long as two chunks, 4 us).
+constexpr int ATTN8_START = 2, ATTN8_NEWEST = 2;
+__device__ __forceinline__ int attn8_units(int len, int page) {
+  const int full = len / page * page;
+  return ATTN8_START + attn8_full_chunks(full) + (len - full + 15) / 16 * ATTN8_NEWEST;
+}
+// first chunk that begins at or after unit u of a row tile with `fullc` chunks of full blocks
+__device__ __forceinline__ int attn8_chunk_at(int u, int fullc) {
+  u -= ATTN8_START;
+  return u <= 0 ? 0 : u <= fullc ? u : fullc + (u - fullc + ATTN8_NEWEST - 1) / ATTN8_NEWEST;
 }
 
-template <int D, int NT>
+// SMALL: pages of 16 tokens, so that a chunk has two.
+template <int D, int NT, bool SMALL>
 struct Attn8Warp {
   using C = Attn8Cfg<D, NT>;
   const Attn8Params& p;
-  const uint32_t ring;   // shared address of this warp's ring
-  const uint8_t* ringp;
+  uint8_t* const ring;
+  uint64_t* const bars;      // one a stage
+  volatile int* const abort_flag;
+  int issued, taken;         // chunks copied and consumed so far (stage and phase follow)
+  bool ok;                   // false: a copy never arrived
   const int lane, g, t;
+  const uint32_t lane_k, lane_v;  // this lane's byte offsets in a half chunk of K and of V
   Attn8Seg s;
   uint32_t qb[D / 16][NT][2];
   float qf[NT][2];       // score factor of this lane's columns: scale * log2(e) * row factor
@@ -131,11 +141,18 @@ struct Attn8Warp {
   int lo_lim, hi_lim;    // least and most of the tile's rows
   float m[NT][2], l[NT][2];
   float acc[D / 16][NT][4];
-  int window, page_now, page_next;  // block of lane 0; page ids of 32 blocks from there, and of the next 32
+  // the copies' window: block of lane 0; page ids of 32 blocks from there, and of the next 32
+  int window, page_now, page_next;
+  size_t newest_at;  // of the newest block's values of this head
+  // the products' window, at most one behind: scales of its 32 blocks, and those of the copies' window
+  int swindow;
+  float ks_now, vs_now, ks_next, vs_next;
 
-  __device__ Attn8Warp(const Attn8Params& pp, uint8_t* smem, int warp_in_cta)
-      : p(pp), ring(smem_u32(smem) + warp_in_cta * C::RING), ringp(smem + warp_in_cta * C::RING),
-        lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3) {}
+  __device__ Attn8Warp(const Attn8Params& pp, uint8_t* smem, int w)
+      : p(pp), ring(smem + w * C::RING), bars(reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + w * C::STAGES),
+        abort_flag(reinterpret_cast<volatile int*>(smem + C::BAR_OFF + C::WARPS * C::STAGES * 8)), issued(0), taken(0),
+        ok(true), lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3),
+        lane_k((4 * (g >> 1) + (g & 1)) * D + t * C::CB), lane_v(t * 4 * D + 16 * g) {}
 
   __device__ __forceinline__ const uint16_t* row_ptr(int r, bool& ok) const {
     const int group = p.heads / p.c.kv_heads, i = r / group;
@@ -148,7 +165,24 @@ struct Attn8Warp {
     return 4 * C::CB * (j / WPC) + C::CB * t + 4 * (j % WPC);
   }
 
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+      }
+#pragma unroll
+    for (int a = 0; a < D / 16; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[a][n][e] = 0.f;
+  }
+
   __device__ __forceinline__ void load_rows() {
+    clear();
     const int group = p.heads / p.c.kv_heads;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -188,19 +222,11 @@ struct Attn8Warp {
         qf[n][e] = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4) * p.scale_log2;
         const int i = (s.rt * C::ROWS + 8 * n + 2 * t + e) / group;
         lim[n][e] = i < s.q_len ? max(0, s.len - s.q_len + i + 1) : 0;
-        m[n][e] = -INFINITY;
-        l[n][e] = 0.f;
       }
     }
     const int i0 = s.rt * C::ROWS / group, i1 = min(s.q_len - 1, (s.rt * C::ROWS + C::ROWS - 1) / group);
     lo_lim = max(0, s.len - s.q_len + i0 + 1);
     hi_lim = max(0, s.len - s.q_len + i1 + 1);
-#pragma unroll
-    for (int a = 0; a < D / 16; ++a)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[a][n][e] = 0.f;
   }
 
   __device__ __forceinline__ int fetch_page(int blk) {
@@ -213,64 +239,84 @@ struct Attn8Warp {
     }
     return id;
   }
+  __device__ __forceinline__ void fetch_scales() {
+    const size_t ph = static_cast<size_t>(page_now) * p.c.kv_heads + s.head;
+    ks_next = __ldg(p.c.k_scale + ph);
+    vs_next = __ldg(p.c.v_scale + ph);
+  }
   __device__ __forceinline__ void open_window(int blk) {
-    window = blk;
+    window = swindow = blk;
     page_now = fetch_page(blk + lane);
     page_next = fetch_page(blk + 32 + lane);
+    fetch_scales();
+    ks_now = ks_next;
+    vs_now = vs_next;
   }
-  __device__ __forceinline__ size_t page_head(int blk) {
+  // byte offset of a block of this head in the pools
+  __device__ __forceinline__ size_t block_at(int blk) {
     if (blk >= window + 32) {
       window += 32;
       page_now = page_next;
       page_next = fetch_page(window + 32 + lane);
+      fetch_scales();
     }
-    return static_cast<size_t>(__shfl_sync(0xffffffffu, page_now, blk - window)) * p.c.kv_heads + s.head;
+    const size_t page = __shfl_sync(0xffffffffu, page_now, blk - window);
+    return (page * p.c.kv_heads + s.head) * static_cast<uint32_t>(p.c.page * D);
+  }
+  __device__ __forceinline__ void block_scales(int blk, float& ks, float& vs) {
+    if (blk >= swindow + 32) {
+      swindow += 32;
+      ks_now = ks_next;
+      vs_now = vs_next;
+    }
+    ks = __shfl_sync(0xffffffffu, ks_now, blk - swindow);
+    vs = __shfl_sync(0xffffffffu, vs_now, blk - swindow);
   }
 
-  // start the copies of chunk c (of full blocks); chunks come in order
-  __device__ __forceinline__ void issue_k(int c, int slot) {
-    const int P = p.c.page;
-    const uint32_t dst = ring + slot * C::STAGE;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int tok = c * ATTN8_CHUNK + 16 * h;
-      const bool live = tok < s.full_tokens;
-      const size_t ph = page_head((live ? tok : c * ATTN8_CHUNK) / P);
-      const uint8_t* src = p.c.k_pages + ph * P * D + (tok % P) * D;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = 4 * (g >> 1) + (g & 1) + 2 * r;
-#pragma unroll
-        for (int x = 0; x < C::NCH; ++x)
-          copy_async<C::CB>(dst + (((h * 2 + r) * C::NCH + x) * 32 + lane) * C::CB, src + row * D + (4 * x + t) * C::CB,
-                            live);
+  // start the copy of chunk c to the next stage; chunks come in order
+  __device__ __forceinline__ void issue(int c, int fullc) {
+    uint8_t* dst = ring + issued % C::STAGES * C::STAGE;
+    uint64_t* bar = bars + issued % C::STAGES;
+    ++issued;
+    if (c >= fullc) {
+      if (lane == 0) {
+        const size_t at = newest_at + static_cast<uint32_t>((c - fullc) * 16 * D);
+        mbar_arrive_expect_tx(bar, C::STAGE);
+        bulk_load(dst, p.c.k_new + at, C::K_BYTES, bar);
+        bulk_load(dst + C::K_BYTES, p.c.v_new + at, C::K_BYTES, bar);
       }
-      copy_async<4>(dst + C::K_BYTES + C::V_BYTES + (h * 32 + lane) * 4, p.c.k_scale + ph, live);
+      return;
     }
-    copy_commit();
-  }
-  __device__ __forceinline__ void issue_v(int c, int slot) {
-    const int P = p.c.page;
-    const uint32_t dst = ring + slot * C::STAGE + C::K_BYTES;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int tok = c * ATTN8_CHUNK + 16 * h;
-      const bool live = tok < s.full_tokens;
-      const size_t ph = page_head((live ? tok : c * ATTN8_CHUNK) / P);
-      const uint8_t* src = p.c.v_pages + ph * P * D + (tok % P) * D;
-#pragma unroll
-      for (int x = 0; x < D / 32; ++x)
-        copy_async<16>(dst + ((h * (D / 32) + x) * 32 + lane) * 16, src + t * 4 * D + 128 * x + 16 * g, live);
-      copy_async<4>(dst + C::V_BYTES + ((2 + h) * 32 + lane) * 4, p.c.v_scale + ph, live);
+    if constexpr (SMALL) {
+      // a half past the full blocks keeps what the stage held: any byte is a code, and its keys are masked
+      const bool both = c * ATTN8_CHUNK + 16 < s.full_tokens;
+      const size_t a0 = block_at(2 * c), a1 = block_at(both ? 2 * c + 1 : 2 * c);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, both ? 64 * D : 32 * D);
+        bulk_load(dst, p.c.k_pages + a0, 16 * D, bar);
+        bulk_load(dst + C::K_BYTES, p.c.v_pages + a0, 16 * D, bar);
+        if (both) {
+          bulk_load(dst + 16 * D, p.c.k_pages + a1, 16 * D, bar);
+          bulk_load(dst + C::K_BYTES + 16 * D, p.c.v_pages + a1, 16 * D, bar);
+        }
+      }
+    } else {
+      const int tok = c * ATTN8_CHUNK;
+      const size_t at = block_at(tok / p.c.page) + static_cast<uint32_t>(tok % p.c.page * D);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, C::STAGE);
+        bulk_load(dst, p.c.k_pages + at, C::K_BYTES, bar);
+        bulk_load(dst + C::K_BYTES, p.c.v_pages + at, C::K_BYTES, bar);
+      }
     }
-    copy_commit();
   }
 
   // scores of one chunk (log2 units, keys outside the rows' view at -inf) -> P (fp32) and the running maximum
-  __device__ __forceinline__ void softmax_step(float (&sc)[2][NT][4], int tok0, bool masked) {
+  template <int H>
+  __device__ __forceinline__ void softmax_step(float (&sc)[H][NT][4], int tok0, bool masked) {
     if (masked) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -285,7 +331,8 @@ struct Attn8Warp {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
+        float x = fmaxf(sc[0][n][e], sc[0][n][e + 2]);
+        if constexpr (H == 2) x = fmaxf(x, fmaxf(sc[1][n][e], sc[1][n][e + 2]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -296,7 +343,7 @@ struct Attn8Warp {
         m[n][e] = now;
         float sum = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             float& v = sc[h][n][e + 2 * r];
@@ -315,233 +362,194 @@ struct Attn8Warp {
     }
   }
 
-  __device__ __forceinline__ void chunk_scores(int c, int slot, float (&sc)[2][NT][4]) {
-    const uint8_t* src = ringp + slot * C::STAGE;
+  __device__ __forceinline__ void chunk_scores(const uint8_t* src, const float (&ks)[2], float (&sc)[2][NT][4]) {
+    uint32_t kw[2][2][D / 16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t w[2][D / 16];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int x = 0; x < C::NCH; ++x) {
-          const uint8_t* at = src + (((h * 2 + r) * C::NCH + x) * 32 + lane) * C::CB;
+          const uint8_t* at = src + 16 * h * D + lane_k + 2 * r * D + 4 * x * C::CB;
           if constexpr (C::CB == 16) {
             const uint4 v = *reinterpret_cast<const uint4*>(at);
-            w[r][4 * x] = v.x; w[r][4 * x + 1] = v.y; w[r][4 * x + 2] = v.z; w[r][4 * x + 3] = v.w;
+            kw[h][r][4 * x] = v.x; kw[h][r][4 * x + 1] = v.y; kw[h][r][4 * x + 2] = v.z; kw[h][r][4 * x + 3] = v.w;
           } else {
             const uint2 v = *reinterpret_cast<const uint2*>(at);
-            w[r][2 * x] = v.x; w[r][2 * x + 1] = v.y;
+            kw[h][r][2 * x] = v.x; kw[h][r][2 * x + 1] = v.y;
           }
         }
-      const float ks = *reinterpret_cast<const float*>(src + C::K_BYTES + C::V_BYTES + (h * 32 + lane) * 4);
+    // each step's product waits for the one before it in the same sum: four sums side by side (two halves of the
+    // chunk, even and odd steps)
+    float odd[2][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[h][n][e] = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
+      for (int h = 0; h < 2; ++h) {
         uint32_t a[4];
-        widen(w[0][j], a[0], a[2]);
-        widen(w[1][j], a[1], a[3]);
+        widen(kw[h][0][j], a[0], a[2]);
+        widen(kw[h][1][j], a[1], a[3]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(sc[h][n], a, qb[j][n][0], qb[j][n][1]);
+        for (int n = 0; n < NT; ++n) {
+          float (&to)[4] = j & 1 ? odd[h][n] : sc[h][n];
+          if (j < 2) mma_f16_first(to, a, qb[j][n][0], qb[j][n][1]);
+          else mma_f16(to, a, qb[j][n][0], qb[j][n][1]);
+        }
       }
 #pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[h][n][e] *= ks * qf[n][e & 1];
-    }
+        for (int e = 0; e < 4; ++e) sc[h][n][e] = (sc[h][n][e] + odd[h][n][e]) * (ks[SMALL ? h : 0] * qf[n][e & 1]);
   }
 
-  __device__ __forceinline__ void chunk_values(int c, int slot, const float (&pr)[2][NT][4], bool masked) {
-    const uint8_t* src = ringp + slot * C::STAGE + C::K_BYTES;
+  __device__ __forceinline__ void chunk_values(const uint8_t* src, const float (&vs)[2], int c, const float (&pr)[2][NT][4], bool masked) {
     uint32_t b[2][NT][2];
     float f[2][NT][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float vs = *reinterpret_cast<const float*>(src + C::V_BYTES + ((2 + h) * 32 + lane) * 4);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         b[h][n][0] = transpose8x8(pack_half2(pr[h][n][0], pr[h][n][1]));
         b[h][n][1] = transpose8x8(pack_half2(pr[h][n][2], pr[h][n][3]));
 #pragma unroll
         for (int e = 0; e < 2; ++e)  // a block that a row does not see adds nothing, whatever its scale
-          f[h][n][e] = masked && lim[n][e] <= c * ATTN8_CHUNK + 16 * h ? 0.f : vs;
+          f[h][n][e] = masked && lim[n][e] <= c * ATTN8_CHUNK + 16 * h ? 0.f : vs[SMALL ? h : 0];
       }
     }
-    const bool one = p.c.page >= ATTN8_CHUNK;  // one scale for the chunk
+    constexpr int XG = D == 128 ? (NT == 1 ? 2 : 1) : D == 64 && NT == 2 ? 1 : D / 32;  // 32-channel groups at a time: as many sums side by side
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) {
-      uint4 w[2];
+    for (int x0 = 0; x0 < D / 32; x0 += XG) {
+      float o[2 * XG][NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) w[h] = *reinterpret_cast<const uint4*>(src + ((h * (D / 32) + x) * 32 + lane) * 16);
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float o[NT][4];
+        for (int x = 0; x < XG; ++x) {
+          const uint4 w = *reinterpret_cast<const uint4*>(src + C::K_BYTES + 16 * h * D + lane_v + 128 * (x0 + x));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a[4];
-          widen(y ? w[h].z : w[h].x, a[0], a[2]);
-          widen(y ? w[h].w : w[h].y, a[1], a[3]);
-          if (h == 0 || !one) {
+          for (int y = 0; y < 2; ++y) {
+            uint32_t a[4];
+            widen(y ? w.z : w.x, a[0], a[2]);
+            widen(y ? w.w : w.y, a[1], a[3]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+            for (int n = 0; n < NT; ++n) {
+              if (h == 0 || SMALL) mma_f16_first(o[2 * x + y][n], a, b[h][n][0], b[h][n][1]);
+              else mma_f16(o[2 * x + y][n], a, b[h][n][0], b[h][n][1]);
+            }
           }
+        }
+        if (h == 1 || SMALL) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(o[n], a, b[h][n][0], b[h][n][1]);
-          if (h == 1 || !one) {
+          for (int x = 0; x < 2 * XG; ++x)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                acc[2 * x + y][n][e] = fmaf(o[n][e], f[one ? 0 : h][n][e & 1], acc[2 * x + y][n][e]);
-          }
+                acc[2 * x0 + x][n][e] = fmaf(o[x][n][e], f[SMALL ? h : 0][n][e & 1], acc[2 * x0 + x][n][e]);
         }
       }
     }
   }
 
-  // a chunk of the newest block, 16-bit values from global memory
+  // 16 tokens of the newest block, 16-bit values
   template <bool BF16>
-  __device__ __forceinline__ void newest_chunk(int c) {
-    const int P = p.c.page, tok0 = s.full_tokens + c * ATTN8_CHUNK, off = c * ATTN8_CHUNK;
-    const int row = p.c.rows ? __ldg(p.c.rows + s.b) : s.b;
-    if (row < 0 || row >= p.c.new_rows) {
-      record_error(DERR_KV_RANGE);
-      return;
-    }
-    const size_t base =
-        ((static_cast<size_t>(row) * 2 + (s.full_tokens / P & 1)) * p.c.kv_heads + s.head) * static_cast<size_t>(P) * D;
-    float sc[2][NT][4];
+  __device__ __forceinline__ void newest_chunk(const uint8_t* src, int tok0) {
+    float sc[1][NT][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[h][n][e] = 0.f;
-    // rows in their own type for the scores: bf16 rows are read again
+      for (int e = 0; e < 4; ++e) sc[0][n][e] = 0.f;
 #pragma unroll
     for (int j = 0; j < D / 16; j += 2) {
-      uint4 w[2][2];
+      uint4 w[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int at = off + 16 * h + 4 * (g >> 1) + (g & 1) + 2 * r;
-          w[h][r] = tok0 - off + at < s.len ? *reinterpret_cast<const uint4*>(p.c.k_new + base + at * D + chan(j))
-                                            : make_uint4(0, 0, 0, 0);
-        }
+      for (int r = 0; r < 2; ++r)
+        w[r] = *reinterpret_cast<const uint4*>(src + ((4 * (g >> 1) + (g & 1) + 2 * r) * D + chan(j)) * 2);
+      const uint32_t a0[4] = {w[0].x, w[1].x, w[0].y, w[1].y};
+      const uint32_t a1[4] = {w[0].z, w[1].z, w[0].w, w[1].w};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        uint4 q = make_uint4(qb[j][n][0], qb[j][n][1], qb[j + 1][n][0], qb[j + 1][n][1]);
-        if constexpr (BF16) {
-          bool ok;
-          const uint16_t* src = row_ptr(s.rt * C::ROWS + 8 * n + g, ok);
-          const uint2 q0 = *reinterpret_cast<const uint2*>(src + chan(j));
-          const uint2 q1 = *reinterpret_cast<const uint2*>(src + chan(j + 1));
-          q = ok ? make_uint4(q0.x, q0.y, q1.x, q1.y) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t a0[4] = {w[h][0].x, w[h][1].x, w[h][0].y, w[h][1].y};
-          const uint32_t a1[4] = {w[h][0].z, w[h][1].z, w[h][0].w, w[h][1].w};
-          if constexpr (BF16) {
-            mma_bf16(sc[h][n], a0, q.x, q.y);
-            mma_bf16(sc[h][n], a1, q.z, q.w);
-          } else {
-            mma_f16(sc[h][n], a0, q.x, q.y);
-            mma_f16(sc[h][n], a1, q.z, q.w);
-          }
+        if constexpr (BF16) {  // rows in their own type: read again
+          bool live;
+          const uint16_t* from = row_ptr(s.rt * C::ROWS + 8 * n + g, live) + chan(j);
+          uint2 q0 = __ldg(reinterpret_cast<const uint2*>(from)), q1 = __ldg(reinterpret_cast<const uint2*>(from + 4));
+          if (!live) q0 = q1 = make_uint2(0, 0);
+          mma_bf16(sc[0][n], a0, q0.x, q0.y);
+          mma_bf16(sc[0][n], a1, q1.x, q1.y);
+        } else {
+          mma_f16(sc[0][n], a0, qb[j][n][0], qb[j][n][1]);
+          mma_f16(sc[0][n], a1, qb[j + 1][n][0], qb[j + 1][n][1]);
         }
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[h][n][e] *= BF16 ? p.scale_log2 : qf[n][e & 1];
-    const bool masked = tok0 + ATTN8_CHUNK > lo_lim;
+      for (int e = 0; e < 4; ++e) sc[0][n][e] *= BF16 ? p.scale_log2 : qf[n][e & 1];
+    const bool masked = tok0 + 16 > lo_lim;
     softmax_step(sc, tok0, masked);
-    uint32_t b[2][NT][2], bl[2][NT][2];
+    uint32_t b[NT][2], bl[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float x = sc[h][n][2 * r], y = sc[h][n][2 * r + 1];
-          if constexpr (BF16) {
-            // bf16 weights keep 8 bits: a second product adds what the first leaves out
-            const uint32_t xh = f_to_h16(x, 1), yh = f_to_h16(y, 1);
-            const uint32_t xl = f_to_h16(x - h16_to_f(xh, 1), 1), yl = f_to_h16(y - h16_to_f(yh, 1), 1);
-            b[h][n][r] = transpose8x8(xh | yh << 16);
-            bl[h][n][r] = transpose8x8(xl | yl << 16);
-          } else {
-            b[h][n][r] = transpose8x8(pack_half2(x, y));
-          }
+      for (int r = 0; r < 2; ++r) {
+        const float x = sc[0][n][2 * r], y = sc[0][n][2 * r + 1];
+        if constexpr (BF16) {
+          // bf16 weights keep 8 bits: a second product adds what the first leaves out
+          const uint32_t xh = f_to_h16(x, 1), yh = f_to_h16(y, 1);
+          const uint32_t xl = f_to_h16(x - h16_to_f(xh, 1), 1), yl = f_to_h16(y - h16_to_f(yh, 1), 1);
+          b[n][r] = transpose8x8(xh | yh << 16);
+          bl[n][r] = transpose8x8(xl | yl << 16);
+        } else {
+          b[n][r] = transpose8x8(pack_half2(x, y));
         }
+      }
+    // of this lane's four tokens, the first `have`
+    auto keep = [&](uint4& v, int have) {
+      const uint32_t k0 = have >= 2 ? 0xffffffffu : have == 1 ? 0xffffu : 0u;
+      const uint32_t k1 = have >= 4 ? 0xffffffffu : have == 3 ? 0xffffu : 0u;
+      v.x &= k0; v.z &= k0; v.y &= k1; v.w &= k1;
+    };
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) {
-      uint4 w[2][2];
+      uint4 w[2];
       bool odd = false;  // an infinity or NaN among the values
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int have = s.len - (tok0 + 16 * h + 4 * t);  // of this lane's four tokens
-        const uint32_t k0 = have >= 2 ? 0xffffffffu : have == 1 ? 0xffffu : 0u;
-        const uint32_t k1 = have >= 4 ? 0xffffffffu : have == 3 ? 0xffffu : 0u;
-        const uint16_t* src = p.c.v_new + base + (static_cast<size_t>(off / 4 + 4 * h + t) * D + 32 * x + 4 * g) * 4;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint4 v = have > 0 ? *reinterpret_cast<const uint4*>(src + 8 * y) : make_uint4(0, 0, 0, 0);
-          v.x &= k0; v.z &= k0; v.y &= k1; v.w &= k1;  // what lies past the end is never summed
-          w[h][y] = v;
-          constexpr uint32_t inf = BF16 ? 0x7f80u : 0x7c00u;
-          const uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                                        __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-          odd |= (top & 0xffffu) >= inf || (top >> 16) >= inf;
-        }
+      for (int y = 0; y < 2; ++y) {
+        w[y] = *reinterpret_cast<const uint4*>(src + C::K_BYTES + (t * D + 32 * x + 4 * g) * 8 + 16 * y);
+        keep(w[y], s.len - (tok0 + 4 * t));  // what lies past the end is never summed
+        constexpr uint32_t inf = BF16 ? 0x7f80u : 0x7c00u;
+        const uint32_t top = __vmaxu2(__vmaxu2(w[y].x & 0x7fff7fffu, w[y].y & 0x7fff7fffu),
+                                      __vmaxu2(w[y].z & 0x7fff7fffu, w[y].w & 0x7fff7fffu));
+        odd |= (top & 0xffffu) >= inf || (top >> 16) >= inf;
       }
       // 0 * infinity must not reach rows that do not see the value: rows are then taken apart by what they see
       const bool strange = __any_sync(0xffffffffu, odd), apart = masked && strange;
-      for (int seen = apart ? max(lo_lim, tok0 + 1) : hi_lim; seen <= max(hi_lim, apart ? tok0 + 1 : 0); ++seen) {
+      for (int seen = apart ? max(lo_lim, tok0 + 1) : hi_lim; seen <= hi_lim; ++seen) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          float o[NT][4];
+          uint4 v = w[y];
+          if (apart) keep(v, seen - (tok0 + 4 * t));
+          const uint32_t a[4] = {v.x, v.z, v.y, v.w};
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            float o[4];
+            if constexpr (BF16) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+              for (int e = 0; e < 4; ++e) o[e] = 0.f;
+              mma_bf16(o, a, b[n][0], b[n][1]);
+              uint32_t al[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint4 v = w[h][y];
-            if (apart) {
-              const int have = seen - (tok0 + 16 * h + 4 * t);
-              const uint32_t k0 = have >= 2 ? 0xffffffffu : have == 1 ? 0xffffu : 0u;
-              const uint32_t k1 = have >= 4 ? 0xffffffffu : have == 3 ? 0xffffu : 0u;
-              v.x &= k0; v.z &= k0; v.y &= k1; v.w &= k1;
+              for (int e = 0; e < 4; ++e) al[e] = strange ? finite_only(a[e]) : a[e];
+              mma_bf16(o, al, bl[n][0], bl[n][1]);
+            } else {
+              mma_f16_first(o, a, b[n][0], b[n][1]);
             }
-            const uint32_t a[4] = {v.x, v.z, v.y, v.w};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if constexpr (BF16) {
-                mma_bf16(o[n], a, b[h][n][0], b[h][n][1]);
-                uint32_t al[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) al[e] = strange ? finite_only(a[e]) : a[e];
-                mma_bf16(o[n], al, bl[h][n][0], bl[h][n][1]);
-              } else {
-                mma_f16(o[n], a, b[h][n][0], b[h][n][1]);
-              }
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (!apart || lim[n][e & 1] == seen) acc[2 * x + y][n][e] += o[n][e];
+              if (!apart || lim[n][e & 1] == seen) acc[2 * x + y][n][e] += o[e];
+          }
         }
       }
     }
@@ -549,51 +557,66 @@ struct Attn8Warp {
 
   // chunks [c0, c1) of the segment
   __device__ __forceinline__ void stream(int c0, int c1) {
-    const int fullc = (s.full_tokens + ATTN8_CHUNK - 1) / ATTN8_CHUNK;
-    const int e1 = min(min(c1, fullc), (hi_lim + ATTN8_CHUNK - 1) / ATTN8_CHUNK);  // what no row sees is not read
-    if (c0 < e1) {
-      open_window(c0 * ATTN8_CHUNK / p.c.page);
-      for (int i = 0; i < ATTN8_STAGES - 1; ++i) {
-        if (c0 + i < e1) {
-          issue_k(c0 + i, i);
-          issue_v(c0 + i, i);
+    const int fullc = attn8_full_chunks(s.full_tokens);
+    // what no row sees is not read
+    const int seen = hi_lim <= s.full_tokens ? attn8_full_chunks(hi_lim) : fullc + (hi_lim - s.full_tokens + 15) / 16;
+    const int e1 = min(c1, seen);
+    if (c0 >= e1) return;
+    newest_at = 0;
+    if (e1 > fullc) {
+      const int row = p.c.rows ? __ldg(p.c.rows + s.b) : s.b;
+      if (row < 0 || row >= p.c.new_rows) {
+        record_error(DERR_KV_RANGE);
+        return;
+      }
+      newest_at = ((static_cast<size_t>(row) * 2 + (s.full_tokens / p.c.page & 1)) * p.c.kv_heads + s.head) *
+                  static_cast<uint32_t>(p.c.page * D);
+    }
+    open_window(c0 * ATTN8_CHUNK / p.c.page);
+    int next = c0;
+    while (next < e1 && next < c0 + C::STAGES - 1) issue(next++, fullc);
+    for (int c = c0; c < e1; ++c) {
+      __syncwarp();  // every lane has read the stage that is filled again
+      if (next < e1) issue(next++, fullc);
+      const int tok0 = c * ATTN8_CHUNK, stage = taken % C::STAGES;
+      float ks[2], vs[2];
+      if (c < fullc) {
+        if constexpr (SMALL) {
+          const bool both = tok0 + 16 < s.full_tokens;
+          block_scales(2 * c, ks[0], vs[0]);
+          block_scales(both ? 2 * c + 1 : 2 * c, ks[1], vs[1]);
         } else {
-          copy_commit();
-          copy_commit();
+          block_scales(tok0 / p.c.page, ks[0], vs[0]);
         }
       }
-      int slot = 0;
-      for (int c = c0; c < e1; ++c) {
-        const int ahead = c + ATTN8_STAGES - 1, aslot = slot == 0 ? ATTN8_STAGES - 1 : slot - 1;
-        float sc[2][NT][4];
-        copy_wait<2 * (ATTN8_STAGES - 1) - 1>();
-        chunk_scores(c, slot, sc);
-        if (ahead < e1) issue_k(ahead, aslot); else copy_commit();
-        const int tok0 = c * ATTN8_CHUNK;
-        const bool masked = min(tok0 + ATTN8_CHUNK, s.full_tokens) > lo_lim || tok0 + ATTN8_CHUNK > s.full_tokens;
-        softmax_step_full(sc, tok0, masked);
-        copy_wait<2 * (ATTN8_STAGES - 1) - 1>();
-        chunk_values(c, slot, sc, masked);
-        if (ahead < e1) issue_v(ahead, aslot); else copy_commit();
-        slot = slot + 1 == ATTN8_STAGES ? 0 : slot + 1;
+      if (!mbar_wait_warp(bars + stage, taken / C::STAGES & 1, abort_flag, DERR_WAIT_TMA)) {
+        // what is in flight must land before the shared memory is anyone else's
+        for (int i = taken; i < issued; ++i) mbar_wait_drain(bars + i % C::STAGES, i / C::STAGES & 1);
+        ok = false;
+        return;
       }
-      copy_wait<0>();
-    }
-    for (int c = max(c0, fullc); c < c1; ++c) {
-      if (s.full_tokens + (c - fullc) * ATTN8_CHUNK >= hi_lim) break;
-      if (p.c.bf16) newest_chunk<true>(c - fullc);
-      else newest_chunk<false>(c - fullc);
-    }
-  }
-  // the last chunk of the full blocks may be half empty: its other half belongs to the newest block
-  __device__ __forceinline__ void softmax_step_full(float (&sc)[2][NT][4], int tok0, bool masked) {
-    if (tok0 + ATTN8_CHUNK > s.full_tokens) {
+      ++taken;
+      const uint8_t* src = ring + stage * C::STAGE;
+      if (c < fullc) {
+        const bool masked = min(tok0 + ATTN8_CHUNK, s.full_tokens) > lo_lim;
+        float sc[2][NT][4];
+        chunk_scores(src, ks, sc);
+        if (SMALL && tok0 + ATTN8_CHUNK > s.full_tokens) {
+          // the chunk's other half belongs to the newest block
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[1][n][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) sc[1][n][e] = -INFINITY;
+        }
+        softmax_step(sc, tok0, masked);
+        chunk_values(src, vs, c, sc, masked);
+      } else if (p.c.bf16) {
+        newest_chunk<true>(src, s.full_tokens + (c - fullc) * 16);
+      } else {
+        newest_chunk<false>(src, s.full_tokens + (c - fullc) * 16);
+      }
     }
-    softmax_step(sc, tok0, masked);
+    __syncwarp();
   }
 
   __device__ __forceinline__ void join_lanes() {
@@ -627,20 +650,19 @@ struct Attn8Warp {
         }
       }
   }
-  __device__ __forceinline__ void leave_part(int warp, int slot) {
+  // (max, sum, accumulator) to [rows][D] at `acc_to` and [rows][2] at `ml_to`
+  __device__ __forceinline__ void leave_part(float* acc_to, float* ml_to) {
     join_lanes();
-    const size_t at = (static_cast<size_t>(warp) * 2 + slot) * C::ROWS;
-    float* ml = p.part + static_cast<size_t>(p.warps) * 2 * C::ROWS * D;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const size_t r = at + 8 * n + 2 * t + e;
+        const int r = 8 * n + 2 * t + e;
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
-          *reinterpret_cast<float4*>(p.part + r * D + 32 * x + 4 * g) =
+          *reinterpret_cast<float4*>(acc_to + r * D + 32 * x + 4 * g) =
               make_float4(acc[2 * x][n][e], acc[2 * x][n][e + 2], acc[2 * x + 1][n][e], acc[2 * x + 1][n][e + 2]);
-        if (g == 0) *reinterpret_cast<float2*>(ml + 2 * r) = make_float2(m[n][e], l[n][e]);
+        if (g == 0) *reinterpret_cast<float2*>(ml_to + 2 * r) = make_float2(m[n][e], l[n][e]);
       }
   }
 };
@@ -656,23 +678,26 @@ __device__ __forceinline__ void attn8_sequence(const Attn8Params& p, int b, int&
   }
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * ATTN8_WARPS, D == 128 ? 1 : 2) k_attn8(const Attn8Params p) {
+template <int D, int NT, bool SMALL>
+__global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const Attn8Params p) {
   using C = Attn8Cfg<D, NT>;
-  extern __shared__ uint8_t smem_attn8[];
-  __shared__ int tot[ATTN8_WARPS];
-  int* line = reinterpret_cast<int*>(smem_attn8 + C::SMEM);  // [batch + 1] first work unit of each sequence
-  griddep_sync();
+  extern __shared__ __align__(128) uint8_t smem_attn8[];
+  __shared__ int tot[C::WARPS], held[C::WARPS], held_slot[C::WARPS];
+  int* line = reinterpret_cast<int*>(smem_attn8 + C::TOTAL);  // [batch + 1] first work unit of each sequence
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  if (tid < C::WARPS * C::STAGES) mbar_init(reinterpret_cast<uint64_t*>(smem_attn8 + C::BAR_OFF) + tid, 1);
+  if (tid == 0) *reinterpret_cast<volatile int*>(smem_attn8 + C::BAR_OFF + C::WARPS * C::STAGES * 8) = 0;
+  fence_mbar_init();
+  griddep_sync();
   const int group = p.heads / p.c.kv_heads;
   int base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32 * ATTN8_WARPS) {
+  for (int b0 = 0; b0 < p.batch; b0 += 32 * C::WARPS) {
     const int b = b0 + tid;
     int n = 0;
     if (b < p.batch) {
       int t0, q_len, len;
       attn8_sequence(p, b, t0, q_len, len);
-      n = p.c.kv_heads * ((q_len * group + C::ROWS - 1) / C::ROWS) * (p.split ? attn8_chunks(len, p.c.page) : 1);
+      n = p.c.kv_heads * ((q_len * group + C::ROWS - 1) / C::ROWS) * (p.split ? attn8_units(len, p.c.page) : 1);
     }
     int sum = n;
 #pragma unroll
@@ -683,7 +708,7 @@ __global__ void __launch_bounds__(32 * ATTN8_WARPS, D == 128 ? 1 : 2) k_attn8(co
     if (lane == 31) tot[wid] = sum;
     __syncthreads();
     int before = base;
-    for (int i = 0; i < ATTN8_WARPS; ++i) {
+    for (int i = 0; i < C::WARPS; ++i) {
       if (i < wid) before += tot[i];
       base += tot[i];
     }
@@ -693,21 +718,23 @@ __global__ void __launch_bounds__(32 * ATTN8_WARPS, D == 128 ? 1 : 2) k_attn8(co
   if (tid == 0) line[p.batch] = base;
   __syncthreads();
   if (p.split && blockIdx.x == 0)
-    for (int i = tid; i <= p.batch; i += 32 * ATTN8_WARPS) p.plan[i] = line[i];
+    for (int i = tid; i <= p.batch; i += 32 * C::WARPS) p.plan[i] = line[i];
 
-  Attn8Warp<D, NT> w(p, smem_attn8, wid);
-  const int warp = blockIdx.x * ATTN8_WARPS + wid;
+  Attn8Warp<D, NT, SMALL> w(p, smem_attn8, wid);
+  const int warp = blockIdx.x * C::WARPS + wid;
   const int per = (base + p.warps - 1) / p.warps;
   int at = p.split ? warp * per : warp;
   const int end = p.split ? min(base, at + per) : base;
-  int b = 0;
-  while (at < end) {
-    b = warp_search(p.batch, at, [&](int i) { return line[i]; });
+  float* const ml = p.part + static_cast<size_t>(p.warps) * 2 * C::ROWS * D;
+  int tile_at = -1;  // of the row tile whose part the warp holds at its end: its first unit on the line
+  int tile_slot = 0;
+  while (w.ok && at < end) {
+    const int b = warp_search(p.batch, at, [&](int i) { return line[i]; });
     int t0, q_len, len;
     attn8_sequence(p, b, t0, q_len, len);
     const int tiles = (q_len * group + C::ROWS - 1) / C::ROWS;
-    const int chunks = p.split ? attn8_chunks(len, p.c.page) : 1;
-    const int item = (at - line[b]) / chunks, c0 = (at - line[b]) % chunks;
+    const int units = p.split ? attn8_units(len, p.c.page) : 1;
+    const int item = (at - line[b]) / units, u0 = (at - line[b]) % units;
     w.s.b = b;
     w.s.head = item / tiles;
     w.s.rt = item % tiles;
@@ -715,29 +742,83 @@ __global__ void __launch_bounds__(32 * ATTN8_WARPS, D == 128 ? 1 : 2) k_attn8(co
     w.s.full_tokens = len / p.c.page * p.c.page;
     w.s.q_len = q_len;
     w.s.t0 = t0;
-    w.load_rows();
-    if (p.split) {
-      const int c1 = min(chunks, c0 + end - at);
-      w.stream(c0, c1);
-      if (c0 == 0 && c1 == chunks) w.finish();
-      else w.leave_part(warp, c0 == 0 ? 1 : 0);
-      at += c1 - c0;
-    } else {
+    if (!p.split) {
+      w.load_rows();
       w.stream(0, attn8_chunks(len, p.c.page));
       w.finish();
       at += p.warps;
+      continue;
     }
+    const int u1 = min(units, u0 + end - at), fullc = attn8_full_chunks(w.s.full_tokens);
+    const int c0 = attn8_chunk_at(u0, fullc), c1 = attn8_chunk_at(u1, fullc);
+    if (c0 < c1 || units == u1 - u0) {
+      w.load_rows();
+      w.stream(c0, c1);
+    } else {
+      w.clear();
+    }
+    if (u0 == 0 && u1 == units) {
+      w.finish();
+    } else if (at + u1 - u0 == end) {
+      tile_at = at - u0;  // the warp ends here: its neighbours may hold the same tile's other parts
+      tile_slot = u0 == 0 ? 1 : 0;
+    } else {
+      const size_t place = static_cast<size_t>(warp) * 2 * C::ROWS;
+      w.leave_part(p.part + place * D, ml + 2 * place);
+    }
+    at += u1 - u0;
+  }
+  if (!p.split) return;
+
+  // The parts that the CTA's warps end with, neighbours of one tile added up in the place of the run's first warp.
+  static_assert(C::RING >= (C::ROWS * D + 2 * C::ROWS) * 4, "a part fits a warp's ring");
+  float* const mine = reinterpret_cast<float*>(smem_attn8 + wid * C::RING);
+  if (tile_at >= 0) w.leave_part(mine, mine + C::ROWS * D);
+  if (lane == 0) {
+    held[wid] = tile_at;
+    held_slot[wid] = tile_slot;
+  }
+  __syncthreads();
+  for (int w0 = 0; w0 < C::WARPS;) {
+    int w1 = w0 + 1;
+    if (held[w0] >= 0) {
+      while (w1 < C::WARPS && held[w1] == held[w0]) ++w1;
+      for (int i = tid; i < C::ROWS * (D / 4); i += 32 * C::WARPS) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        auto part = [&](int x) { return reinterpret_cast<const float*>(smem_attn8 + x * C::RING); };
+        float top = -INFINITY;
+        for (int x = w0; x < w1; ++x) top = fmaxf(top, part(x)[C::ROWS * D + 2 * r]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x = w0; x < w1; ++x) {
+          const float f = fast_exp2(part(x)[C::ROWS * D + 2 * r] - ref);
+          const float4 v = *reinterpret_cast<const float4*>(part(x) + r * D + d);
+          sum = fmaf(part(x)[C::ROWS * D + 2 * r + 1], f, sum);
+          o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+        }
+        const size_t to = (static_cast<size_t>(blockIdx.x * C::WARPS + w0) * 2 + held_slot[w0]) * C::ROWS + r;
+        *reinterpret_cast<float4*>(p.part + to * D + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(ml + 2 * to) = make_float2(top, sum);
+      }
+    }
+    w0 = w1;
   }
 }
 
-// Adds the parts of the row tiles that several warps share, in the warps' order.
-// blockIdx.x: a place for every row tile (n rows make at most n / ROWS + 1 tiles),
-// blockIdx.y: key head.
+// Adds the parts of the row tiles that several CTAs (or two places of one) share, in a fixed order.  blockIdx.x: a
+// place for every row tile (n rows make at most n / ROWS + 1 tiles), blockIdx.y: key head.  Latency is all there is
+// to it: the parts' maxima and sums come in one round of loads, the accumulators in another.
+constexpr int ATTN8_JOIN_THREADS = 256;
+
 template <int D, int NT>
-__global__ void __launch_bounds__(128) k_attn8_join(const Attn8Params p) {
+__global__ void __launch_bounds__(ATTN8_JOIN_THREADS) k_attn8_join(const Attn8Params p) {
   using C = Attn8Cfg<D, NT>;
+  constexpr int V4 = D / 4, T = ATTN8_JOIN_THREADS, MOST = 160;  // parts: one a CTA and one more
+  __shared__ float2 mls[MOST * C::ROWS];
+  __shared__ float4 red[T];
   griddep_sync();
-  const int group = p.heads / p.c.kv_heads, u = blockIdx.x;
+  const int group = p.heads / p.c.kv_heads, u = blockIdx.x, tid = threadIdx.x;
   const int b = warp_search(p.batch, u, [&](int i) {
     return static_cast<int>(static_cast<long long>(__ldg(p.cu + i)) * group / C::ROWS) + i;
   });
@@ -746,37 +827,62 @@ __global__ void __launch_bounds__(128) k_attn8_join(const Attn8Params p) {
   const int rt = u - (static_cast<int>(static_cast<long long>(__ldg(p.cu + b)) * group / C::ROWS) + b);
   const int tiles = (q_len * group + C::ROWS - 1) / C::ROWS;
   if (rt < 0 || rt >= tiles) return;
-  const int chunks = attn8_chunks(len, p.c.page);
-  const int per = (p.plan[p.batch] + p.warps - 1) / p.warps;
-  const int first = p.plan[b] + (blockIdx.y * tiles + rt) * chunks;
-  const int w0 = first / per, w1 = (first + chunks - 1) / per;
+  const int units = attn8_units(len, p.c.page), total = p.plan[p.batch];
+  const int per = (total + p.warps - 1) / p.warps;
+  const int first = p.plan[b] + (blockIdx.y * tiles + rt) * units;
+  const int w0 = first / per, w1 = (first + units - 1) / per;
   if (w0 == w1) return;
+  // A CTA's run of parts is in the place of its first warp; the last part is its warp's own if more follows it.
+  const int cta0 = w0 / C::WARPS, cta1 = w1 / C::WARPS;
+  const bool own = first + units != min(total, (w1 + 1) * per) && w1 % C::WARPS != 0;
+  const int parts = cta1 - cta0 + 1 + own, rows = min(C::ROWS, q_len * group - rt * C::ROWS);
   const float* ml = p.part + static_cast<size_t>(p.warps) * 2 * C::ROWS * D;
-  for (int i = threadIdx.x; i < C::ROWS * (D / 4); i += 128) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    const int row = rt * C::ROWS + r, tok = row / group;
-    if (tok >= q_len) continue;
-    float top = -INFINITY;
-    for (int w = w0; w <= w1; ++w) {
-      const size_t at = (static_cast<size_t>(w) * 2 + (w == w0)) * C::ROWS + r;
-      top = fmaxf(top, ml[2 * at]);
-    }
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  auto place = [&](int i) {
+    const int w = i == 0 ? w0 : i > cta1 - cta0 ? w1 : (cta0 + i) * C::WARPS;
+    return (static_cast<size_t>(w) * 2 + (i == 0)) * C::ROWS;  // the part that begins the tile is its warp's second
+  };
+  for (int i = tid; i < parts * rows; i += T) {
+    const int x = i / rows, r = i % rows;
+    mls[i] = *reinterpret_cast<const float2*>(ml + 2 * (place(x) + r));
+  }
+  __syncthreads();
+  const int n = rows * V4;               // (row, four channels) to add up
+  const int lanes = max(1, T / n);       // threads that share one's parts
+  for (int n0 = 0; n0 < n; n0 += T) {
+    const int unit = n0 + tid % min(n, T), sub = n < T ? tid / n : 0;
+    const bool on = unit < n && sub < lanes;
+    const int r = unit / V4, d = unit % V4 * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    if (on) {
+      float top = -INFINITY;
+      for (int x = 0; x < parts; ++x) top = fmaxf(top, mls[x * rows + r].x);
+      const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-    for (int w = w0; w <= w1; ++w) {
-      const size_t at = (static_cast<size_t>(w) * 2 + (w == w0)) * C::ROWS + r;
-      const float f = fast_exp2(ml[2 * at] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(p.part + at * D + d);
-      sum += ml[2 * at + 1] * f;
-      o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
+      for (int x = sub; x < parts; x += lanes) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part + (place(x) + r) * D + d);
+        const float f = fast_exp2(mls[x * rows + r].x - ref);
+        o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+      }
+      for (int x = 0; x < parts; ++x) sum = fmaf(mls[x * rows + r].y, fast_exp2(mls[x * rows + r].x - ref), sum);
     }
-    const float inv = len - q_len + tok >= 0 ? 1.f / sum : 0.f;
-    uint2 out;
-    out.x = f_to_h16(o[0] * inv, p.c.bf16) | f_to_h16(o[1] * inv, p.c.bf16) << 16;
-    out.y = f_to_h16(o[2] * inv, p.c.bf16) | f_to_h16(o[3] * inv, p.c.bf16) << 16;
-    *reinterpret_cast<uint2*>(p.out + (t0 + tok) * p.ld_out +
-                              static_cast<size_t>(blockIdx.y * group + row % group) * D + d) = out;
+    if (lanes > 1) {
+      red[tid] = o;
+      __syncthreads();
+    }
+    if (on && sub == 0) {
+      for (int i = 1; i < lanes; ++i) {
+        const float4 v = red[tid + i * n];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+      }
+      const int row = rt * C::ROWS + r, tok = row / group;
+      const float inv = len - q_len + tok >= 0 ? 1.f / sum : 0.f;
+      uint2 out;
+      out.x = f_to_h16(o.x * inv, p.c.bf16) | f_to_h16(o.y * inv, p.c.bf16) << 16;
+      out.y = f_to_h16(o.z * inv, p.c.bf16) | f_to_h16(o.w * inv, p.c.bf16) << 16;
+      *reinterpret_cast<uint2*>(p.out + (t0 + tok) * p.ld_out +
+                                static_cast<size_t>(blockIdx.y * group + row % group) * D + d) = out;
+    }
   }
 }
 

@@ -100,33 +100,46 @@ int kv8_read_impl(const B200KvCache8* c, const int* cu, const int* start, const 
 
 // Rows of a tile: one column tile of 8 where a key head's rows fit it, else two.
 int attn8_rows(int max_q_len, int group) { return static_cast<long long>(max_q_len) * group <= 8 ? 8 : 16; }
-// CTAs of 8 warps an SM holds (shared memory; head_dim 128 takes all of it)
-int attn8_ctas(int head_dim) { return (head_dim == 128 ? 1 : 2) * num_sms(); }
+template <int D, int NT>
+constexpr size_t attn8_slots() {  // floats of one SM's partial results
+  using C = Attn8Cfg<D, NT>;
+  return static_cast<size_t>(C::WARPS) * 2 * C::ROWS * (D + 2);
+}
 
 size_t attn8_workspace(int batch, int heads, int kv_heads, int head_dim, int max_q_len) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_q_len <= 0) return 0;
-  const size_t slots = static_cast<size_t>(attn8_ctas(head_dim)) * ATTN8_WARPS * 2 * attn8_rows(max_q_len, heads / kv_heads);
-  return slots * (head_dim + 2) * sizeof(float) + (static_cast<size_t>(batch) + 1) * sizeof(int);
+  const bool one = attn8_rows(max_q_len, heads / kv_heads) == 8;
+  const size_t floats = head_dim == 32 ? (one ? attn8_slots<32, 1>() : attn8_slots<32, 2>())
+                        : head_dim == 64 ? (one ? attn8_slots<64, 1>() : attn8_slots<64, 2>())
+                                         : (one ? attn8_slots<128, 1>() : attn8_slots<128, 2>());
+  return num_sms() * floats * sizeof(float) + (static_cast<size_t>(batch) + 1) * sizeof(int);
 }
 
-template <int D, int NT>
-int launch_attn8(Attn8Params& p, int ctas, long long rows, cudaStream_t st) {
+template <int D, int NT, bool SMALL>
+int launch_attn8(Attn8Params& p, long long rows, cudaStream_t st) {
   using C = Attn8Cfg<D, NT>;
-  p.warps = ctas * ATTN8_WARPS;
-  p.plan = reinterpret_cast<int*>(p.part + static_cast<size_t>(p.warps) * 2 * C::ROWS * (D + 2));
+  const int ctas = std::min(num_sms(), 150);  // (the join kernel holds a part a CTA)
+  p.warps = ctas * C::WARPS;
+  p.plan = reinterpret_cast<int*>(p.part + ctas * attn8_slots<D, NT>());
   // whole row tiles keep every warp busy when there are several a warp; else the keys are cut too
   p.split = rows / C::ROWS * p.c.kv_heads < 4LL * p.warps;
-  auto kern = k_attn8<D, NT>;
-  const int smem = C::SMEM + (ATTN8_MAX_BATCH + 1) * 4;
-  if (int rc = set_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
-  launch_kernel(kern, dim3(ctas), dim3(32 * ATTN8_WARPS), C::SMEM + (p.batch + 1) * 4, st, p);
+  auto kern = k_attn8<D, NT, SMALL>;
+  static_assert(C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4 + 128 <= 227 * 1024, "ring and line fit an SM");
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4)) return rc;
+  launch_kernel(kern, dim3(ctas), dim3(32 * C::WARPS), C::TOTAL + (p.batch + 1) * 4, st, p);
   if (int rc = launch_status()) return rc;
   if (p.split) {
-    launch_kernel(k_attn8_join<D, NT>, dim3(static_cast<unsigned>(rows / C::ROWS + p.batch), p.c.kv_heads), dim3(128), 0,
-                  st, p);
+    launch_kernel(k_attn8_join<D, NT>, dim3(static_cast<unsigned>(rows / C::ROWS + p.batch), p.c.kv_heads),
+                  dim3(ATTN8_JOIN_THREADS), 0, st, p);
     return launch_status();
   }
   return B200_OK;
+}
+
+template <int D>
+int launch_attn8_d(Attn8Params& p, bool one, long long rows, cudaStream_t st) {
+  if (p.c.page == 16) return one ? launch_attn8<D, 1, true>(p, rows, st) : launch_attn8<D, 2, true>(p, rows, st);
+  return one ? launch_attn8<D, 1, false>(p, rows, st) : launch_attn8<D, 2, false>(p, rows, st);
 }
 
 int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, long long ld_out, const int* cu,
@@ -141,8 +154,8 @@ int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, 
   if (!al16(q) || !al16(out) || ld_q % 8 || ld_out % 8) return B200_ERR_ALIGN;
   const int group = heads / c->kv_heads;
   const long long rows = static_cast<long long>(tokens) * group;
-  // the line of (sequence, head, row tile, chunk) work is numbered in 32 bits
-  const long long chunks = static_cast<long long>(c->table_width) * c->page_size / ATTN8_CHUNK + 2;
+  // the line of (sequence, head, row tile, unit) work is numbered in 32 bits
+  const long long chunks = static_cast<long long>(c->table_width) * c->page_size / ATTN8_CHUNK + 1 + ATTN8_START + 8 * ATTN8_NEWEST;
   if (rows > 0x7fffffffLL || (rows / 8 + c->batch) * c->kv_heads * chunks > 0x7fffffffLL) return B200_ERR_TILE;
   if (!ws || ws_bytes < attn8_workspace(c->batch, heads, c->kv_heads, c->head_dim, max_q_len)) return B200_ERR_WORKSPACE;
   if (!al16(ws)) return B200_ERR_ALIGN;
@@ -160,12 +173,11 @@ int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, 
   p.heads = heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = static_cast<float*>(ws);
-  const int ctas = attn8_ctas(c->head_dim);
   const bool one = attn8_rows(max_q_len, group) == 8;
   switch (c->head_dim) {
-    case 32: return one ? launch_attn8<32, 1>(p, ctas, rows, st) : launch_attn8<32, 2>(p, ctas, rows, st);
-    case 64: return one ? launch_attn8<64, 1>(p, ctas, rows, st) : launch_attn8<64, 2>(p, ctas, rows, st);
-    default: return one ? launch_attn8<128, 1>(p, ctas, rows, st) : launch_attn8<128, 2>(p, ctas, rows, st);
+    case 32: return launch_attn8_d<32>(p, one, rows, st);
+    case 64: return launch_attn8_d<64>(p, one, rows, st);
+    default: return launch_attn8_d<128>(p, one, rows, st);
   }
 }
 

@@ -27,7 +27,7 @@ from torch import Tensor
 from . import runtime as rt
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-MAX_BATCH = 4096
+MAX_BATCH = 2048
 
 
 def _need(ok: bool, what: str) -> None:
