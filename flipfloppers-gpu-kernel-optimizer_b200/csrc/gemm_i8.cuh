@@ -41,17 +41,6 @@ __device__ __forceinline__ void load_row16(const void* x, size_t base, int k, in
   }
 }
 
-// rint(x / s), x / s rounded to fp32 first, for |x| <= 127.5 s.  The product with the reciprocal is within 2^-20 of
-// the quotient's magnitude bound, so only quotients that near a half need the division itself.
-__device__ __forceinline__ float quotient(float x, float s, float inv) {
-  const float y = x * inv, r = rintf(y);
-  return fabsf(fabsf(y - r) - 0.5f) > 2e-3f ? r : rintf(__fdiv_rn(x, s));
-}
-__device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
-  return (static_cast<uint32_t>(static_cast<int>(a)) & 0xffu) | (static_cast<uint32_t>(static_cast<int>(b)) & 0xffu) << 8 |
-         (static_cast<uint32_t>(static_cast<int>(c)) & 0xffu) << 16 | static_cast<uint32_t>(static_cast<int>(d)) << 24;
-}
-
 // x [M, K] (row stride ldx elements) -> codes int8 [M, ldq], scale [M].  A row with an
 // infinity or NaN gets a NaN scale, so its outputs are NaN.  TPR threads a row (a warp
 // for rows up to 2048 values); the row is read twice, the second time from L1.
@@ -87,20 +76,21 @@ __global__ void __launch_bounds__(256) k_quant_rows(const void* x, long long ldx
   for (int k = tid * 16; k < K; k += TPR * 16) {
     float v[16];
     load_row16<DT>(x, base, k, K, vec && k + 16 <= K, v);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float r = !live ? 0.f : small ? rintf(__fdiv_rn(v[j], s)) : quotient(v[j], s, inv);
-      v[j] = fminf(fmaxf(r, -127.f), 127.f);
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (live) {
+      w.x = quantize4(v[0], v[1], v[2], v[3], s, inv, small);
+      w.y = quantize4(v[4], v[5], v[6], v[7], s, inv, small);
+      w.z = quantize4(v[8], v[9], v[10], v[11], s, inv, small);
+      w.w = quantize4(v[12], v[13], v[14], v[15], s, inv, small);
     }
-    uint4 w = make_uint4(pack_codes(v[0], v[1], v[2], v[3]), pack_codes(v[4], v[5], v[6], v[7]),
-                         pack_codes(v[8], v[9], v[10], v[11]), pack_codes(v[12], v[13], v[14], v[15]));
     int8_t* to = q + row * ldq + k;
     if (k + 16 <= ldq && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
       *reinterpret_cast<uint4*>(to) = w;
     } else {
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (k + j < K) to[j] = static_cast<int8_t>(v[j]);
+        if (k + j < K) to[j] = static_cast<int8_t>(x[j >> 2] >> (8 * (j & 3)));
     }
   }
 }

@@ -51,6 +51,8 @@ struct Kv8AppendParams {
   int rot, interleaved, rope_rows;
   int tokens, batch, heads;
   int by_token;          // unit = token (few tokens a sequence) instead of unit = block
+  unsigned row_recip, q_recip;  // 2^32 / (units of a row), 2^32 / q_each, rounded up (q_each 1: 0)
+  int k_each, q_each;    // key heads of K, and query heads, that a CTA takes one after another
 };
 
 __device__ __forceinline__ float h16_to_f(uint32_t bits, int bf16) {
@@ -91,40 +93,221 @@ __device__ __forceinline__ int warp_search(int n, int u, F key) {
   return lo;
 }
 
-// Eight channels of one head of one token at position pos, from d, rotated.
-__device__ __forceinline__ uint4 rotate8(const Kv8AppendParams& p, const uint16_t* row, int d, int pos) {
-  const uint4 w = *reinterpret_cast<const uint4*>(row + d);
-  if (p.cos == nullptr || d >= p.rot) return w;
-  const int half = p.rot >> 1;
+// Four codes rint(x / s) as signed bytes, x / s rounded to fp32 first; inv = 1 / s, |x| <= 127.5 s unless `divide`.
+// t = x * inv + 1.5 * 2^23 has the nearest whole number in its low bits; x * inv is within 2^-15 of the quotient, so
+// only quotients that near a half (and scales whose reciprocal could overflow: `divide`) need the division itself.
+__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d, float s, float inv, bool divide) {
+  const float magic = 12582912.f;
+  const float x[4] = {a, b, c, d};
+  float t[4], near = 1.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = fmaf(x[i], inv, magic);
+    near = fminf(near, fabsf(fabsf(fmaf(x[i], inv, magic - t[i])) - 0.5f));
+  }
+  if (divide || near < 2e-3f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f) + magic;
+  }
+  return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                     __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+}
+// i / d for i * d < 2^32, with d's reciprocal 2^32 / d rounded up (d >= 2)
+__device__ __forceinline__ int over(int i, unsigned recip) { return static_cast<int>(__umulhi(i, recip)); }
+
+// The rotation of one row (a head of a token at position pos) falls into units: a pair of 8-channel vectors
+// (i, i + rot/2) that turn together, or a vector on its own (interleaved pairs, channels past rot).
+struct Kv8Unit {
+  uint4 a, b;
+  int da, db;  // first channels; db < 0: one vector only
+};
+__device__ __forceinline__ int kv8_units(const Kv8AppendParams& p) {
+  return (p.c.head_dim >> 3) - (p.interleaved ? 0 : p.rot >> 4);
+}
+__device__ __forceinline__ void load8(const float* from, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = __ldg(reinterpret_cast<const float4*>(from) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ Kv8Unit rotate_unit(const Kv8AppendParams& p, const uint16_t* row, int i, int pos) {
+  Kv8Unit u;
+  u.db = -1;
+  const int half = p.rot >> 1, bf16 = p.c.bf16;
   const float* cs = p.cos + static_cast<size_t>(pos) * half;
   const float* sn = p.sin + static_cast<size_t>(pos) * half;
   float x[8], y[8];
-  unpack8(w, p.c.bf16, x);
-  if (p.interleaved) {  // pairs (2i, 2i + 1)
+  if (p.interleaved) {
+    u.da = 8 * i;
+    u.a = __ldg(reinterpret_cast<const uint4*>(row + u.da));
+    if (u.da < p.rot) {
+      const float4 co = __ldg(reinterpret_cast<const float4*>(cs + u.da / 2));
+      const float4 si = __ldg(reinterpret_cast<const float4*>(sn + u.da / 2));
+      const float c4[4] = {co.x, co.y, co.z, co.w}, s4[4] = {si.x, si.y, si.z, si.w};
+      unpack8(u.a, bf16, x);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float co = __ldg(cs + (d + i) / 2), si = __ldg(sn + (d + i) / 2);
-      y[i] = __fsub_rn(__fmul_rn(x[i], co), __fmul_rn(x[i + 1], si));
-      y[i + 1] = __fadd_rn(__fmul_rn(x[i + 1], co), __fmul_rn(x[i], si));
+      for (int j = 0; j < 8; j += 2) {
+        y[j] = __fsub_rn(__fmul_rn(x[j], c4[j / 2]), __fmul_rn(x[j + 1], s4[j / 2]));
+        y[j + 1] = __fadd_rn(__fmul_rn(x[j + 1], c4[j / 2]), __fmul_rn(x[j], s4[j / 2]));
+      }
+      u.a = pack8(y, bf16);
     }
-  } else {  // pairs (i, i + rot/2)
-    const bool second = d >= half;
-    float o[8];
-    unpack8(*reinterpret_cast<const uint4*>(row + (second ? d - half : d + half)), p.c.bf16, o);
-    const int f = second ? d - half : d;
+  } else if (i < p.rot >> 4) {
+    u.da = 8 * i;
+    u.db = 8 * i + half;
+    u.a = __ldg(reinterpret_cast<const uint4*>(row + u.da));
+    u.b = __ldg(reinterpret_cast<const uint4*>(row + u.db));
+    float co[8], si[8], z[8], w[8];
+    load8(cs + u.da, co);
+    load8(sn + u.da, si);
+    unpack8(u.a, bf16, x);
+    unpack8(u.b, bf16, y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float co = __ldg(cs + f + i), si = __ldg(sn + f + i);
-      const float a = __fmul_rn(x[i], co), b = __fmul_rn(o[i], si);
-      y[i] = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
+    for (int j = 0; j < 8; ++j) {
+      z[j] = __fsub_rn(__fmul_rn(x[j], co[j]), __fmul_rn(y[j], si[j]));
+      w[j] = __fadd_rn(__fmul_rn(y[j], co[j]), __fmul_rn(x[j], si[j]));
+    }
+    u.a = pack8(z, bf16);
+    u.b = pack8(w, bf16);
+  } else {
+    u.da = 8 * (i + (p.rot >> 4));
+    u.a = __ldg(reinterpret_cast<const uint4*>(row + u.da));
+  }
+  return u;
+}
+
+// One block of K (what 0) or V (what 1) of one key head: new tokens [lo, hi), `had` earlier ones.
+__device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int what, int head, int nrow, int blk, int lo,
+                                                  int hi, int first, int last, int had, int len, bool full, bool keep,
+                                                  int page, const uint16_t* rows, uint16_t* tile, unsigned* top_bits) {
+  const Kv8Cache& c = p.c;
+  const int tid = threadIdx.x, nth = blockDim.x, D = c.head_dim, P = c.page, per_row = kv8_units(p);
+  uint4* const tile16 = reinterpret_cast<uint4*>(tile);
+  uint16_t* newest = (what ? c.v_new : c.k_new) +
+                     ((static_cast<size_t>(nrow) * 2 + (blk & 1)) * c.kv_heads + head) * P * D;
+  unsigned top = 0;  // largest |value| as 16 bits: their order is the values' order, NaN above infinity
+  auto see = [&](uint32_t x) { top = __vmaxu2(top, x & 0x7fff7fffu); };
+  const size_t hoff = static_cast<size_t>(p.heads + (what ? c.kv_heads : 0) + head) * D;
+  // tokens [from, to) of the block that begins at position `begin`: to the tile and to the newest blocks
+  auto take = [&](int begin, int from, int to, bool to_tile, bool to_newest) {
+    if (what == 0) {
+      for (int i = tid; i < (to - from) * per_row; i += nth) {
+        const int row = over(i, p.row_recip), pos = from + row, at = pos - begin;
+        const Kv8Unit x = rotate_unit(p, rows + pos * p.ld + hoff, i - row * per_row, pos);
+        auto put = [&](uint4 w, int d) {
+          if (to_tile) {
+            *reinterpret_cast<uint4*>(tile + at * D + d) = w;
+            see(w.x); see(w.y); see(w.z); see(w.w);
+          }
+          if (to_newest) *reinterpret_cast<uint4*>(newest + at * D + d) = w;
+        };
+        put(x.a, x.da);
+        if (x.db >= 0) put(x.b, x.db);
+      }
+      return;
+    }
+    // four tokens of eight channels: the rows' vectors, transposed to the layout of V
+    const int g0 = (from - begin) >> 2, groups = ((to - begin + 3) >> 2) - g0, vpr = D >> 3, vsh = __ffs(vpr) - 1;
+    for (int i = tid; i < groups * vpr; i += nth) {
+      const int grp = g0 + (i >> vsh), d = (i & (vpr - 1)) * 8, pos = begin + 4 * grp;
+      uint32_t r[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (pos + k >= from && pos + k < to)
+          w = __ldg(reinterpret_cast<const uint4*>(rows + (pos + k) * p.ld + hoff + d));
+        r[k][0] = w.x; r[k][1] = w.y; r[k][2] = w.z; r[k][3] = w.w;
+        see(w.x); see(w.y); see(w.z); see(w.w);
+      }
+      uint16_t* dst[2] = {tile + (grp * D + d) * 4, newest + (grp * D + d) * 4};
+      const bool on[2] = {to_tile, to_newest};
+      const bool whole = pos >= from && pos + 4 <= to;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (!on[x]) continue;
+        if (whole) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)  // channels d + 2w, d + 2w + 1
+            *reinterpret_cast<uint4*>(dst[x] + 8 * w) =
+                make_uint4(__byte_perm(r[0][w], r[1][w], 0x5410), __byte_perm(r[2][w], r[3][w], 0x5410),
+                           __byte_perm(r[0][w], r[1][w], 0x7632), __byte_perm(r[2][w], r[3][w], 0x7632));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (pos + k >= from && pos + k < to)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) dst[x][4 * j + k] = static_cast<uint16_t>(r[k][j >> 1] >> (16 * (j & 1)));
+        }
+      }
+    }
+  };
+  take(blk * P, lo, hi, full, keep);
+  if (!full) return;
+  // the block's earlier tokens
+  if (what == 0) {
+    for (int i = tid; i < had * (D >> 3); i += nth) {
+      const uint4 w = reinterpret_cast<const uint4*>(newest)[i];
+      tile16[i] = w;
+      see(w.x); see(w.y); see(w.z); see(w.w);
+    }
+  } else {
+    for (int i = tid; i < ((had + 3) >> 2) * (D >> 1); i += nth) {  // four tokens of two channels
+      uint4 w = reinterpret_cast<const uint4*>(newest)[i];
+      const int keep4 = had - i / (D >> 1) * 4;  // of the four, the earlier ones
+      if (keep4 >= 4) {
+        tile16[i] = w;
+      } else {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          if (k < keep4) {
+            tile[8 * i + k] = static_cast<uint16_t>(x[k >> 1] >> (16 * (k & 1)));
+            tile[8 * i + 4 + k] = static_cast<uint16_t>(x[2 + (k >> 1)] >> (16 * (k & 1)));
+          }
+        const uint32_t k0 = keep4 >= 2 ? 0xffffffffu : 0xffffu, k1 = keep4 == 3 ? 0xffffu : 0u;
+        w.x &= k0; w.z &= k0; w.y &= k1; w.w &= k1;
+      }
+      see(w.x); see(w.y); see(w.z); see(w.w);
     }
   }
-  return pack8(y, p.c.bf16);
+  const int after = last - ((last - blk) & 1);  // the kept block of this slot
+  const unsigned mine = top;
+  if (blk == first && had > 0 && after >= first + 2) {
+    __syncthreads();
+    take(after * P, after * P, min(len, (after + 1) * P), false, true);
+  }
+  top = max(mine & 0xffffu, mine >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) top_bits[tid >> 5] = top;
+  __syncthreads();
+  for (int i = 0; i < (nth >> 5); ++i) top = max(top, top_bits[i]);
+  const float amax = h16_to_f(top, c.bf16);
+  const float scale = amax < INFINITY ? __fmul_rn(amax, 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+  const size_t ph = static_cast<size_t>(page) * c.kv_heads + head;
+  if (tid == 0) (what ? c.v_scale : c.k_scale)[ph] = scale;
+  const bool live = scale > 0.f;      // false for an all-zero block and for NaN: codes are then zero points
+  const bool small = scale < 1e-30f;  // 1 / scale could overflow: divide
+  const float inv = __fdiv_rn(1.f, scale);
+  uint4* out = reinterpret_cast<uint4*>((what ? c.v_pages : c.k_pages) + ph * P * D);
+  for (int i = tid; i < P * D / 16; i += nth) {
+    uint32_t w[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};  // the zero point
+    if (live) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        unpack8(tile16[2 * i + h], c.bf16, v);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[2 * h + j] ^= quantize4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], scale, inv, small);
+      }
+    }
+    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // Unit = one touched block of one sequence.  blockIdx.x: unit (or token, by_token);
-// blockIdx.y = 3 * head + {0: K, 1: V, 2: the head's group of query heads}.
-// Memory-bound; shared memory holds the block's 16-bit values between the
+// blockIdx.y: k_each heads of K, a head of V, or q_each query heads.
+// Memory-bound.  Heads of one CTA share the rows of cos and sin through L1 (with a head a CTA they came from L2 for
+// every head, twice the bytes of the head itself: 114 us against 77 us for 27000 tokens of 16 + 2 x 16 heads).  Shared memory holds the block's 16-bit values, in the order of the page's codes, between the
 // maximum and the codes, so that nothing is read twice.
 __global__ void __launch_bounds__(256) k_kv8_append(const Kv8AppendParams p) {
   extern __shared__ uint4 smem_kv8[];
@@ -132,8 +315,9 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8AppendParams p) {
   griddep_sync();
   const Kv8Cache& c = p.c;
   const int tid = threadIdx.x, nth = blockDim.x;
-  const int D = c.head_dim, P = c.page, head = blockIdx.y / 3, what = blockIdx.y % 3;
-  const int u = blockIdx.x;
+  const int D = c.head_dim, P = c.page, u = blockIdx.x;
+  const int k_ctas = (c.kv_heads + p.k_each - 1) / p.k_each;
+  const int y = blockIdx.y, what = y < k_ctas ? 0 : y < k_ctas + c.kv_heads ? 1 : 2;
   int b, blk;
   if (p.by_token) {
     b = warp_search(p.batch, u, [&](int i) { return __ldg(p.cu + i); });
@@ -156,122 +340,41 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8AppendParams p) {
     if (tid == 0) record_error(DERR_KV_RANGE);
     return;
   }
-  const int vpr = D >> 3, vsh = __ffs(vpr) - 1;  // 16-byte vectors a row (a power of two)
   const uint16_t* rows = p.qkv + (t0 - start) * p.ld;  // row of position 0
+  const int per_row = kv8_units(p);
 
-  if (what == 2) {  // the query heads of this key head's group
-    const int group = p.heads / c.kv_heads, per = group * vpr;
-    for (int i = tid; i < (hi - lo) * per; i += nth) {
-      const int pos = lo + i / per, r = i % per, h = head * group + (r >> vsh), d = (r & (vpr - 1)) * 8;
-      const uint16_t* src = rows + pos * p.ld + static_cast<size_t>(h) * D;
-      *reinterpret_cast<uint4*>(p.q_out + (static_cast<size_t>(t0 + pos - start) * p.heads + h) * D + d) =
-          rotate8(p, src, d, pos);
+  if (what == 2) {
+    const int h0 = (y - k_ctas - c.kv_heads) * p.q_each, h1 = min(p.heads, h0 + p.q_each);
+    for (int i = tid; i < (hi - lo) * p.q_each * per_row; i += nth) {
+      const int row = over(i, p.row_recip), at = p.q_each > 1 ? over(row, p.q_recip) : row;
+      const int pos = lo + at, h = h0 + row - at * p.q_each;
+      if (h >= h1) continue;
+      const Kv8Unit x = rotate_unit(p, rows + pos * p.ld + static_cast<size_t>(h) * D, i - row * per_row, pos);
+      uint16_t* to = p.q_out + (static_cast<size_t>(t0 + pos - start) * p.heads + h) * D;
+      *reinterpret_cast<uint4*>(to + x.da) = x.a;
+      if (x.db >= 0) *reinterpret_cast<uint4*>(to + x.db) = x.b;
     }
     return;
   }
 
   const bool full = hi == (blk + 1) * P;
-  const bool keep = blk >= (len - 1) / P - 1;
-  uint16_t* newest = (what ? c.v_new : c.k_new) +
-                     ((static_cast<size_t>(nrow) * 2 + (blk & 1)) * c.kv_heads + head) * P * D;
-  const uint16_t* tile = reinterpret_cast<const uint16_t*>(smem_kv8);
-  unsigned top = 0;  // largest |value| as 16 bits: their order is the values' order, NaN above infinity
-  auto see = [&](uint4 w) {
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, x[i] & 0x7fff7fffu);
-  };
-  const size_t hoff = static_cast<size_t>(p.heads + (what ? c.kv_heads : 0) + head) * D;
-  auto load = [&](int pos, int d) {
-    const uint16_t* src = rows + pos * p.ld + hoff;
-    return what ? *reinterpret_cast<const uint4*>(src + d) : rotate8(p, src, d, pos);
-  };
-  auto put_newest = [&](int at, int d, uint4 w) {
-    if (what) {
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-      uint16_t* to = newest + ((at >> 2) * D + d) * 4 + (at & 3);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) to[4 * j] = static_cast<uint16_t>(x[j >> 1] >> (16 * (j & 1)));
-    } else {
-      *reinterpret_cast<uint4*>(newest + at * D + d) = w;
-    }
-  };
-  // The first touched block may have its earlier tokens in the slot that a later
-  // kept block of the same parity takes over: the first block's CTA then writes
-  // that block's values too, after it has read what it needs.
-  const int first = start / P, last = (len - 1) / P, had0 = start - first * P;
-  const bool others = had0 > 0 && blk >= first + 2 && ((blk - first) & 1) == 0;
-  for (int i = tid; i < (hi - lo) * vpr; i += nth) {
-    const int pos = lo + (i >> vsh), d = (i & (vpr - 1)) * 8, at = pos - blk * P;
-    if (!full && (!keep || others)) break;
-    const uint4 w = load(pos, d);
-    if (full) {
-      smem_kv8[at * vpr + (d >> 3)] = w;
-      see(w);
-    }
-    if (keep && !others) put_newest(at, d, w);
-  }
-  if (!full) return;
-  // the block's earlier tokens, from the newest blocks
-  const int had = lo - blk * P;
-  if (what == 0) {
-    for (int i = tid; i < had * vpr; i += nth) {
-      const uint4 w = *reinterpret_cast<const uint4*>(newest + i * 8);
-      smem_kv8[i] = w;
-      see(w);
-    }
-  } else {
-    uint16_t* t16 = reinterpret_cast<uint16_t*>(smem_kv8);
-    for (int i = tid; i < had * D; i += nth) {
-      const int at = i / D, d = i % D;
-      const uint32_t x = newest[((at >> 2) * D + d) * 4 + (at & 3)];
-      t16[i] = static_cast<uint16_t>(x);
-      top = __vmaxu2(top, x & 0x7fffu);
-    }
-  }
-  const int after = last - ((last - blk) & 1);  // the kept block of this slot
-  if (blk == first && had > 0 && after >= first + 2) {
-    __syncthreads();
-    const int from = after * P, to = min(len, from + P);
-    for (int i = tid; i < (to - from) * vpr; i += nth) {
-      const int d = (i & (vpr - 1)) * 8, at = i >> vsh;
-      put_newest(at, d, load(from + at, d));
-    }
-  }
-  top = max(top & 0xffffu, top >> 16);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) top_bits[tid >> 5] = top;
-  __syncthreads();
-  for (int i = 0; i < (nth >> 5); ++i) top = max(top, top_bits[i]);
-  const float amax = h16_to_f(top, c.bf16);
-  const float scale = amax < INFINITY ? __fmul_rn(amax, 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
-  const int page = __ldg(c.table + static_cast<size_t>(b) * c.table_width + blk);
+  const int page = full ? __ldg(c.table + static_cast<size_t>(b) * c.table_width + blk) : 0;
   if (page < 0 || page >= c.num_pages) {
     if (tid == 0) record_error(DERR_KV_RANGE);
     return;
   }
-  const size_t ph = static_cast<size_t>(page) * c.kv_heads + head;
-  if (tid == 0) (what ? c.v_scale : c.k_scale)[ph] = scale;
-  const bool live = scale > 0.f;  // false for an all-zero block and for NaN: codes are then zero points
-  auto code = [&](uint32_t bits) -> uint32_t {
-    if (!live) return 128u;
-    const float r = rintf(__fdiv_rn(h16_to_f(bits, c.bf16), scale));
-    return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(r, -127.f), 127.f)) + 128);
-  };
-  uint4* out = reinterpret_cast<uint4*>((what ? c.v_pages : c.k_pages) + ph * P * D);
-  for (int i = tid; i < P * D / 16; i += nth) {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // K: 16 channels of a token; V: four tokens of four channels
-        const int e = what ? ((i * 4 / D) * 4 + k) * D + (i * 4) % D + j : i * 16 + j * 4 + k;
-        w[j] |= code(tile[e]) << (8 * k);
-      }
-    }
-    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  // The newest two blocks keep their 16-bit values.  The first touched block may have its earlier tokens in the slot
+  // that a later kept block of the same parity takes over: the first block's CTA then writes that block's values
+  // too, after it has read what it needs.
+  const int first = start / P, last = (len - 1) / P, had = lo - blk * P;
+  const bool others = start % P != 0 && blk >= first + 2 && ((blk - first) & 1) == 0;
+  const bool keep = blk >= last - 1 && !others;
+  if (!full && !keep) return;
+  const int head0 = what ? y - k_ctas : y * p.k_each, head1 = what ? head0 + 1 : min(c.kv_heads, head0 + p.k_each);
+  uint16_t* tile = reinterpret_cast<uint16_t*>(smem_kv8);
+  for (int head = head0; head < head1; ++head) {
+    if (head > head0) __syncthreads();  // the tile is free again
+    k_kv8_append_head(p, what, head, nrow, blk, lo, hi, first, last, had, len, full, keep, page, rows, tile, top_bits);
   }
 }
 

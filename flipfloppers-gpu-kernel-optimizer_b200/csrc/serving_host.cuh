@@ -50,7 +50,7 @@ int kv8_append_impl(const B200KvCache8* c, const void* qkv, long long ld, void* 
   if (!qkv || !q_out || (cos == nullptr) != (sin == nullptr)) return B200_ERR_ARG;
   if (cos && (rot <= 0 || rot % 16 || rot > c->head_dim || rope_rows <= 0)) return B200_ERR_TILE;
   if (ld < static_cast<long long>(heads + 2 * c->kv_heads) * c->head_dim) return B200_ERR_ARG;
-  if (!al16(qkv) || !al16(q_out) || ld % 8) return B200_ERR_ALIGN;
+  if (!al16(qkv) || !al16(q_out) || !al16(cos) || !al16(sin) || ld % 8) return B200_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   Kv8AppendParams p{};
   p.c = cache8_of(c);
@@ -72,7 +72,17 @@ int kv8_append_impl(const B200KvCache8* c, const void* qkv, long long ld, void* 
   p.by_token = tokens <= by_block;
   const unsigned units = static_cast<unsigned>(p.by_token ? tokens : by_block);
   const int smem = c->page_size * c->head_dim * 2;
-  launch_kernel(k_kv8_append, dim3(units, 3u * c->kv_heads), dim3(p.by_token ? 64 : 256), smem, st, p);
+  // heads a CTA: all that give its threads one unit each for single tokens; for prompts as many as leave every SM
+  // several CTAs
+  const int threads = p.by_token ? 128 : 256, per_row = c->head_dim / 8 - (interleaved ? 0 : p.rot / 16);
+  const bool many = !p.by_token && by_block * c->kv_heads >= 32LL * num_sms();
+  p.k_each = many ? std::min(c->kv_heads, 4) : 1;
+  p.q_each = p.by_token ? std::max(1, threads / per_row) : many ? 8 : 4;
+  p.row_recip = static_cast<unsigned>((0x100000000ull + per_row - 1) / per_row);
+  p.q_recip = p.q_each > 1 ? static_cast<unsigned>((0x100000000ull + p.q_each - 1) / p.q_each) : 0;
+  const unsigned slots = (c->kv_heads + p.k_each - 1) / p.k_each + c->kv_heads + (heads + p.q_each - 1) / p.q_each;
+  if (slots > 65535) return B200_ERR_TILE;
+  launch_kernel(k_kv8_append, dim3(units, slots), dim3(threads), smem, st, p);
   return launch_status();
 }
 
