@@ -26,7 +26,7 @@ __device__ __forceinline__ void load_row16(const void* x, size_t base, int k, in
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float u[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + base + k) + i), DT == DT_BF16, u);
+        unpack8<DT == DT_BF16>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + base + k) + i), u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[8 * i + j] = u[j];
       }
@@ -185,8 +185,7 @@ __device__ __forceinline__ void i8_epilogue(const CUtensorMap* tmO, const GemmI8
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       if constexpr (DT == DT_F32) w[j] = __float_as_uint(v[j]);
-      else if constexpr (DT == DT_F16) w[j] = pack_half2(v[2 * j], v[2 * j + 1]);
-      else w[j] = f_to_h16(v[2 * j], 1) | f_to_h16(v[2 * j + 1], 1) << 16;
+      else w[j] = pack2<DT == DT_BF16>(v[2 * j], v[2 * j + 1]);
     }
     uint8_t* slot = stg + (gc & 1) * 2048;
     if (lane == 0) bulk_wait_read_1();  // the slot's previous chunk has left

@@ -36,6 +36,7 @@ struct Kv8Cache {
   const int* table;      // [batch, table_width] page of each block
   const int* rows;       // [batch] row of the newest-blocks buffers, null = the batch index
   int num_pages, kv_heads, page, head_dim, new_rows, table_width;
+  int page_shift, dim_shift;  // their logarithms
   int bf16;              // 16-bit type: 0 fp16, 1 bf16
 };
 
@@ -52,7 +53,7 @@ struct Kv8AppendParams {
   int tokens, batch, heads;
   int by_token;          // unit = token (few tokens a sequence) instead of unit = block
   unsigned row_recip, q_recip;  // 2^32 / (units of a row), 2^32 / q_each, rounded up (q_each 1: 0)
-  int k_each, q_each;    // key heads of K, and query heads, that a CTA takes one after another
+  int k_each, q_each;    // key heads of K or V that a CTA splits its threads among, query heads that it takes
 };
 
 __device__ __forceinline__ float h16_to_f(uint32_t bits, int bf16) {
@@ -61,19 +62,33 @@ __device__ __forceinline__ float h16_to_f(uint32_t bits, int bf16) {
 __device__ __forceinline__ uint32_t f_to_h16(float v, int bf16) {
   return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
-__device__ __forceinline__ void unpack8(uint4 w, int bf16, float (&v)[8]) {
+template <bool BF16>
+__device__ __forceinline__ void unpack8(uint4 w, float (&v)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[2 * i] = h16_to_f(u[i] & 0xffffu, bf16);
-    v[2 * i + 1] = h16_to_f(u[i] >> 16, bf16);
+    if constexpr (BF16) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
   }
 }
-__device__ __forceinline__ uint4 pack8(const float (&v)[8], int bf16) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = f_to_h16(v[2 * i], bf16) | (f_to_h16(v[2 * i + 1], bf16) << 16);
-  return make_uint4(u[0], u[1], u[2], u[3]);
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_half2(a, b);
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
 }
 
 // Largest b in [0, n) with key(b) <= u, key non-decreasing and key(0) <= u: each
@@ -94,7 +109,7 @@ __device__ __forceinline__ int warp_search(int n, int u, F key) {
 }
 
 // Four codes rint(x / s) as signed bytes, x / s rounded to fp32 first; inv = 1 / s, |x| <= 127.5 s unless `divide`.
-// t = x * inv + 1.5 * 2^23 has the nearest whole number in its low bits; x * inv is within 2^-15 of the quotient, so
+// t = x * inv + 1.5 * 2^23 has the nearest whole number in its low bits; x * inv is within 2^-16 of the quotient, so
 // only quotients that near a half (and scales whose reciprocal could overflow: `divide`) need the division itself.
 __device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d, float s, float inv, bool divide) {
   const float magic = 12582912.f;
@@ -105,7 +120,7 @@ __device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d
     t[i] = fmaf(x[i], inv, magic);
     near = fminf(near, fabsf(fabsf(fmaf(x[i], inv, magic - t[i])) - 0.5f));
   }
-  if (divide || near < 2e-3f) {
+  if (divide || near < 4e-5f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f) + magic;
   }
@@ -129,10 +144,11 @@ __device__ __forceinline__ void load8(const float* from, float (&v)[8]) {
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
+template <bool BF16>
 __device__ __forceinline__ Kv8Unit rotate_unit(const Kv8AppendParams& p, const uint16_t* row, int i, int pos) {
   Kv8Unit u;
   u.db = -1;
-  const int half = p.rot >> 1, bf16 = p.c.bf16;
+  const int half = p.rot >> 1;
   const float* cs = p.cos + static_cast<size_t>(pos) * half;
   const float* sn = p.sin + static_cast<size_t>(pos) * half;
   float x[8], y[8];
@@ -143,13 +159,13 @@ __device__ __forceinline__ Kv8Unit rotate_unit(const Kv8AppendParams& p, const u
       const float4 co = __ldg(reinterpret_cast<const float4*>(cs + u.da / 2));
       const float4 si = __ldg(reinterpret_cast<const float4*>(sn + u.da / 2));
       const float c4[4] = {co.x, co.y, co.z, co.w}, s4[4] = {si.x, si.y, si.z, si.w};
-      unpack8(u.a, bf16, x);
+      unpack8<BF16>(u.a, x);
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         y[j] = __fsub_rn(__fmul_rn(x[j], c4[j / 2]), __fmul_rn(x[j + 1], s4[j / 2]));
         y[j + 1] = __fadd_rn(__fmul_rn(x[j + 1], c4[j / 2]), __fmul_rn(x[j], s4[j / 2]));
       }
-      u.a = pack8(y, bf16);
+      u.a = pack8<BF16>(y);
     }
   } else if (i < p.rot >> 4) {
     u.da = 8 * i;
@@ -159,15 +175,15 @@ __device__ __forceinline__ Kv8Unit rotate_unit(const Kv8AppendParams& p, const u
     float co[8], si[8], z[8], w[8];
     load8(cs + u.da, co);
     load8(sn + u.da, si);
-    unpack8(u.a, bf16, x);
-    unpack8(u.b, bf16, y);
+    unpack8<BF16>(u.a, x);
+    unpack8<BF16>(u.b, y);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       z[j] = __fsub_rn(__fmul_rn(x[j], co[j]), __fmul_rn(y[j], si[j]));
       w[j] = __fadd_rn(__fmul_rn(y[j], co[j]), __fmul_rn(x[j], si[j]));
     }
-    u.a = pack8(z, bf16);
-    u.b = pack8(w, bf16);
+    u.a = pack8<BF16>(z);
+    u.b = pack8<BF16>(w);
   } else {
     u.da = 8 * (i + (p.rot >> 4));
     u.a = __ldg(reinterpret_cast<const uint4*>(row + u.da));
@@ -175,12 +191,15 @@ __device__ __forceinline__ Kv8Unit rotate_unit(const Kv8AppendParams& p, const u
   return u;
 }
 
-// One block of K (what 0) or V (what 1) of one key head: new tokens [lo, hi), `had` earlier ones.
-__device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int what, int head, int nrow, int blk, int lo,
-                                                  int hi, int first, int last, int had, int len, bool full, bool keep,
+// One block of K (what 0) or V (what 1) of one key head (one past the last only joins the barrier): new tokens
+// [lo, hi), `had` earlier ones.
+template <bool BF16>
+__device__ __forceinline__ void kv8_append_head(const Kv8AppendParams& p, int what, int head, int nrow, int blk, int lo,
+                                                int hi, int first, int last, int had, int len, bool full, bool keep,
                                                   int page, const uint16_t* rows, uint16_t* tile, unsigned* top_bits) {
   const Kv8Cache& c = p.c;
-  const int tid = threadIdx.x, nth = blockDim.x, D = c.head_dim, P = c.page, per_row = kv8_units(p);
+  const int nth = blockDim.x / p.k_each, tid = threadIdx.x % nth;  // the head's threads
+  const int D = c.head_dim, P = c.page, per_row = kv8_units(p);
   uint4* const tile16 = reinterpret_cast<uint4*>(tile);
   uint16_t* newest = (what ? c.v_new : c.k_new) +
                      ((static_cast<size_t>(nrow) * 2 + (blk & 1)) * c.kv_heads + head) * P * D;
@@ -192,7 +211,7 @@ __device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int 
     if (what == 0) {
       for (int i = tid; i < (to - from) * per_row; i += nth) {
         const int row = over(i, p.row_recip), pos = from + row, at = pos - begin;
-        const Kv8Unit x = rotate_unit(p, rows + pos * p.ld + hoff, i - row * per_row, pos);
+        const Kv8Unit x = rotate_unit<BF16>(p, rows + pos * p.ld + hoff, i - row * per_row, pos);
         auto put = [&](uint4 w, int d) {
           if (to_tile) {
             *reinterpret_cast<uint4*>(tile + at * D + d) = w;
@@ -240,10 +259,11 @@ __device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int 
       }
     }
   };
-  take(blk * P, lo, hi, full, keep);
+  if (head < c.kv_heads) take(blk * P, lo, hi, full, keep);
   if (!full) return;
   // the block's earlier tokens
-  if (what == 0) {
+  if (head >= c.kv_heads) {
+  } else if (what == 0) {
     for (int i = tid; i < had * (D >> 3); i += nth) {
       const uint4 w = reinterpret_cast<const uint4*>(newest)[i];
       tile16[i] = w;
@@ -252,7 +272,7 @@ __device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int 
   } else {
     for (int i = tid; i < ((had + 3) >> 2) * (D >> 1); i += nth) {  // four tokens of two channels
       uint4 w = reinterpret_cast<const uint4*>(newest)[i];
-      const int keep4 = had - i / (D >> 1) * 4;  // of the four, the earlier ones
+      const int keep4 = had - (i >> (c.dim_shift - 1)) * 4;  // of the four, the earlier ones
       if (keep4 >= 4) {
         tile16[i] = w;
       } else {
@@ -269,19 +289,19 @@ __device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int 
       see(w.x); see(w.y); see(w.z); see(w.w);
     }
   }
-  const int after = last - ((last - blk) & 1);  // the kept block of this slot
-  const unsigned mine = top;
-  if (blk == first && had > 0 && after >= first + 2) {
-    __syncthreads();
-    take(after * P, after * P, min(len, (after + 1) * P), false, true);
-  }
-  top = max(mine & 0xffffu, mine >> 16);
+  top = max(top & 0xffffu, top >> 16);
   top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) top_bits[tid >> 5] = top;
+  if ((tid & 31) == 0) top_bits[threadIdx.x >> 5] = top;
   __syncthreads();
-  for (int i = 0; i < (nth >> 5); ++i) top = max(top, top_bits[i]);
-  const float amax = h16_to_f(top, c.bf16);
+  if (head >= c.kv_heads) return;
+  const int warp0 = (threadIdx.x - tid) >> 5;
+  top = 0;
+  for (int i = 0; i < (nth >> 5); ++i) top = max(top, top_bits[warp0 + i]);
+  const float amax = h16_to_f(top, BF16);
   const float scale = amax < INFINITY ? __fmul_rn(amax, 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+  const int after = last - ((last - blk) & 1);  // the kept block of this slot
+  if (blk == first && had > 0 && after >= first + 2)
+    take(after * P, after * P, min(len, (after + 1) * P), false, true);
   const size_t ph = static_cast<size_t>(page) * c.kv_heads + head;
   if (tid == 0) (what ? c.v_scale : c.k_scale)[ph] = scale;
   const bool live = scale > 0.f;      // false for an all-zero block and for NaN: codes are then zero points
@@ -294,7 +314,7 @@ __device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[8];
-        unpack8(tile16[2 * i + h], c.bf16, v);
+        unpack8<BF16>(tile16[2 * i + h], v);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           w[2 * h + j] ^= quantize4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], scale, inv, small);
@@ -309,26 +329,27 @@ __device__ __forceinline__ void k_kv8_append_head(const Kv8AppendParams& p, int 
 // Memory-bound.  Heads of one CTA share the rows of cos and sin through L1 (with a head a CTA they came from L2 for
 // every head, twice the bytes of the head itself: 114 us against 77 us for 27000 tokens of 16 + 2 x 16 heads).  Shared memory holds the block's 16-bit values, in the order of the page's codes, between the
 // maximum and the codes, so that nothing is read twice.
+template <bool BF16>
 __global__ void __launch_bounds__(256) k_kv8_append(const Kv8AppendParams p) {
   extern __shared__ uint4 smem_kv8[];
   __shared__ unsigned top_bits[8];
   griddep_sync();
   const Kv8Cache& c = p.c;
   const int tid = threadIdx.x, nth = blockDim.x;
-  const int D = c.head_dim, P = c.page, u = blockIdx.x;
+  const int D = c.head_dim, P = c.page, psh = c.page_shift, u = blockIdx.x;
   const int k_ctas = (c.kv_heads + p.k_each - 1) / p.k_each;
-  const int y = blockIdx.y, what = y < k_ctas ? 0 : y < k_ctas + c.kv_heads ? 1 : 2;
+  const int y = blockIdx.y, what = y < k_ctas ? 0 : y < 2 * k_ctas ? 1 : 2;
   int b, blk;
   if (p.by_token) {
     b = warp_search(p.batch, u, [&](int i) { return __ldg(p.cu + i); });
     const int t0 = __ldg(p.cu + b), pos = __ldg(p.start + b) + u - t0;
     // the first token of a block in this call stands for the block
-    if (u < t0 || u >= __ldg(p.cu + b + 1) || (u != t0 && pos % P != 0)) return;
-    blk = pos / P;
+    if (u < t0 || u >= __ldg(p.cu + b + 1) || (u != t0 && (pos & (P - 1)) != 0)) return;
+    blk = pos >> psh;
   } else {
     // n tokens touch at most n/P + 2 blocks, so cu/P + 2b spaces the sequences apart
-    b = warp_search(p.batch, u, [&](int i) { return __ldg(p.cu + i) / P + 2 * i; });
-    blk = __ldg(p.start + b) / P + u - (__ldg(p.cu + b) / P + 2 * b);
+    b = warp_search(p.batch, u, [&](int i) { return (__ldg(p.cu + i) >> psh) + 2 * i; });
+    blk = (__ldg(p.start + b) >> psh) + u - ((__ldg(p.cu + b) >> psh) + 2 * b);
   }
   const int t0 = __ldg(p.cu + b), start = __ldg(p.start + b);
   const int n = __ldg(p.cu + b + 1) - t0, len = start + n;
@@ -344,12 +365,12 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8AppendParams p) {
   const int per_row = kv8_units(p);
 
   if (what == 2) {
-    const int h0 = (y - k_ctas - c.kv_heads) * p.q_each, h1 = min(p.heads, h0 + p.q_each);
+    const int h0 = (y - 2 * k_ctas) * p.q_each, h1 = min(p.heads, h0 + p.q_each);
     for (int i = tid; i < (hi - lo) * p.q_each * per_row; i += nth) {
       const int row = over(i, p.row_recip), at = p.q_each > 1 ? over(row, p.q_recip) : row;
       const int pos = lo + at, h = h0 + row - at * p.q_each;
       if (h >= h1) continue;
-      const Kv8Unit x = rotate_unit(p, rows + pos * p.ld + static_cast<size_t>(h) * D, i - row * per_row, pos);
+      const Kv8Unit x = rotate_unit<BF16>(p, rows + pos * p.ld + static_cast<size_t>(h) * D, i - row * per_row, pos);
       uint16_t* to = p.q_out + (static_cast<size_t>(t0 + pos - start) * p.heads + h) * D;
       *reinterpret_cast<uint4*>(to + x.da) = x.a;
       if (x.db >= 0) *reinterpret_cast<uint4*>(to + x.db) = x.b;
@@ -366,16 +387,13 @@ __global__ void __launch_bounds__(256) k_kv8_append(const Kv8AppendParams p) {
   // The newest two blocks keep their 16-bit values.  The first touched block may have its earlier tokens in the slot
   // that a later kept block of the same parity takes over: the first block's CTA then writes that block's values
   // too, after it has read what it needs.
-  const int first = start / P, last = (len - 1) / P, had = lo - blk * P;
-  const bool others = start % P != 0 && blk >= first + 2 && ((blk - first) & 1) == 0;
+  const int first = start >> psh, last = (len - 1) >> psh, had = lo - blk * P;
+  const bool others = (start & (P - 1)) != 0 && blk >= first + 2 && ((blk - first) & 1) == 0;
   const bool keep = blk >= last - 1 && !others;
   if (!full && !keep) return;
-  const int head0 = what ? y - k_ctas : y * p.k_each, head1 = what ? head0 + 1 : min(c.kv_heads, head0 + p.k_each);
-  uint16_t* tile = reinterpret_cast<uint16_t*>(smem_kv8);
-  for (int head = head0; head < head1; ++head) {
-    if (head > head0) __syncthreads();  // the tile is free again
-    k_kv8_append_head(p, what, head, nrow, blk, lo, hi, first, last, had, len, full, keep, page, rows, tile, top_bits);
-  }
+  const int sub = threadIdx.x / (blockDim.x / p.k_each), head = (what ? y - k_ctas : y) * p.k_each + sub;
+  kv8_append_head<BF16>(p, what, head, nrow, blk, lo, hi, first, last, had, len, full, keep, page, rows,
+                        reinterpret_cast<uint16_t*>(smem_kv8) + sub * P * D, top_bits);
 }
 
 struct Kv8ReadParams {
@@ -390,6 +408,7 @@ struct Kv8ReadParams {
 
 // Windows of tokens as 16-bit rows.  A warp takes four tokens of one head: lanes
 // run along the channels, eight a lane, so rows leave in 16-byte stores.
+template <bool BF16>
 __global__ void __launch_bounds__(256) k_kv8_read(const Kv8ReadParams p) {
   griddep_sync();
   const Kv8Cache& c = p.c;
@@ -402,7 +421,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8ReadParams p) {
   int b = warp_search(p.batch, first, [&](int i) { return __ldg(p.cu + i); });
   if (t >= p.tokens) return;
   while (b + 1 < p.batch && t >= __ldg(p.cu + b + 1)) ++b;
-  const int pos = __ldg(p.start + b) + t - __ldg(p.cu + b), blk = pos / P, at = pos % P;
+  const int pos = __ldg(p.start + b) + t - __ldg(p.cu + b), blk = pos >> c.page_shift, at = pos & (P - 1);
   const int nrow = c.rows ? __ldg(c.rows + b) : b;
   const size_t to = (static_cast<size_t>(t) * c.kv_heads + head) * D + d;
   const bool full = (blk + 1) * P <= __ldg(p.lens + b);
@@ -437,8 +456,8 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8ReadParams p) {
     kf[j] = __fmul_rn(static_cast<float>(static_cast<int>(kc) - 128), ks);
     vf[j] = __fmul_rn(static_cast<float>(static_cast<int>(vc) - 128), vs);
   }
-  *reinterpret_cast<uint4*>(p.k_out + to) = pack8(kf, c.bf16);
-  *reinterpret_cast<uint4*>(p.v_out + to) = pack8(vf, c.bf16);
+  *reinterpret_cast<uint4*>(p.k_out + to) = pack8<BF16>(kf);
+  *reinterpret_cast<uint4*>(p.v_out + to) = pack8<BF16>(vf);
 }
 
 }  // namespace b200

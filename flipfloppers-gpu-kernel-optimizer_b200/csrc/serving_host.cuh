@@ -38,6 +38,8 @@ Kv8Cache cache8_of(const B200KvCache8* a) {
   c.new_rows = a->newest_rows;
   c.table_width = a->table_width;
   c.bf16 = a->bf16 != 0;
+  c.page_shift = __builtin_ctz(a->page_size);
+  c.dim_shift = __builtin_ctz(a->head_dim);
   return c;
 }
 
@@ -71,18 +73,20 @@ int kv8_append_impl(const B200KvCache8* c, const void* qkv, long long ld, void* 
   if (by_block > 0x7fffffffLL) return B200_ERR_TILE;
   p.by_token = tokens <= by_block;
   const unsigned units = static_cast<unsigned>(p.by_token ? tokens : by_block);
-  const int smem = c->page_size * c->head_dim * 2;
-  // heads a CTA: all that give its threads one unit each for single tokens; for prompts as many as leave every SM
-  // several CTAs
+  const int tile = c->page_size * c->head_dim * 2;
+  // heads a CTA: for single tokens one of K and V, and query heads that give its threads a unit each; for prompts as
+  // many as leave every SM several CTAs and the tiles within 48 KB
   const int threads = p.by_token ? 128 : 256, per_row = c->head_dim / 8 - (interleaved ? 0 : p.rot / 16);
-  const bool many = !p.by_token && by_block * c->kv_heads >= 32LL * num_sms();
-  p.k_each = many ? std::min(c->kv_heads, 4) : 1;
+  const bool many = !p.by_token && by_block * c->kv_heads >= 16LL * num_sms();
+  p.k_each = 1;
+  while (many && p.k_each < 4 && 2 * p.k_each <= c->kv_heads && 2 * p.k_each * tile <= 48 * 1024) p.k_each *= 2;
+  const int smem = p.k_each * tile;
   p.q_each = p.by_token ? std::max(1, threads / per_row) : many ? 8 : 4;
   p.row_recip = static_cast<unsigned>((0x100000000ull + per_row - 1) / per_row);
   p.q_recip = p.q_each > 1 ? static_cast<unsigned>((0x100000000ull + p.q_each - 1) / p.q_each) : 0;
-  const unsigned slots = (c->kv_heads + p.k_each - 1) / p.k_each + c->kv_heads + (heads + p.q_each - 1) / p.q_each;
+  const unsigned slots = 2 * ((c->kv_heads + p.k_each - 1) / p.k_each) + (heads + p.q_each - 1) / p.q_each;
   if (slots > 65535) return B200_ERR_TILE;
-  launch_kernel(k_kv8_append, dim3(units, slots), dim3(threads), smem, st, p);
+  launch_kernel(p.c.bf16 ? k_kv8_append<true> : k_kv8_append<false>, dim3(units, slots), dim3(threads), smem, st, p);
   return launch_status();
 }
 
@@ -104,7 +108,7 @@ int kv8_read_impl(const B200KvCache8* c, const int* cu, const int* start, const 
   p.tokens = tokens;
   p.batch = c->batch;
   const int per = 256 / (c->head_dim / 8);
-  launch_kernel(k_kv8_read, dim3((tokens + per - 1) / per, c->kv_heads), dim3(256), 0, st, p);
+  launch_kernel(p.c.bf16 ? k_kv8_read<true> : k_kv8_read<false>, dim3((tokens + per - 1) / per, c->kv_heads), dim3(256), 0, st, p);
   return launch_status();
 }
 
