@@ -18,16 +18,22 @@ be captured in a CUDA graph and replayed with other values in them.
 
 from __future__ import annotations
 
-import math
+import importlib.util
+import os
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
 
+from . import build as _build
 from . import runtime as rt
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-MAX_BATCH = 2048
+
+
+def _on_device(t: Tensor) -> None:
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise RuntimeError("libb200block kernels take CUDA tensors on the current device only (no CPU fallback)")
 
 
 def _need(ok: bool, what: str) -> None:
@@ -35,27 +41,28 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-# The checks of a call cost as much as a small kernel runs: they compare first and put the message together
-# only when one fails.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_f32, _i32 = torch.float32, torch.int32
+_module = None
 
 
-def _stream(index: Optional[int], *ts: Optional[Tensor]) -> int:
-    """The current stream of CUDA device ``index``, which every tensor must be on and which must be current."""
-    for t in ts:
-        if t is not None and (not t.is_cuda or t.get_device() != index):
-            raise RuntimeError("libb200block kernels take CUDA tensors on one device only (no CPU fallback)")
-    if index is None or index < 0 or torch._C._cuda_getDevice() != index:
-        raise RuntimeError(f"tensors are on CUDA device {index}, which is not the current one (no CPU fallback)")
-    return _raw_stream(index)
+def _native():
+    """The calls' C++ side (csrc/serving_binding.cpp); raises if it has not been built."""
+    global _module
+    if _module is None:
+        rt.lib()
+        path = _build.BINDING_PATH
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python {_build.__file__}`")
+        spec = importlib.util.spec_from_file_location("b200serving", path)
+        _module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_module)
+    return _module
 
 
-def _index(t: Tensor, n: int, name: str) -> int:
-    """The address of an index tensor."""
-    if t.dtype != _i32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous int32 tensor with {n} entries expected")
-    return t.data_ptr()
+def _done(result, what: str):
+    """A call's result; a launcher's status raises."""
+    if type(result) is int:
+        rt.check(result, what)
+    return result
 
 
 class PagedKV8:
@@ -74,39 +81,28 @@ class PagedKV8:
 
     def __init__(self, k_pages: Tensor, v_pages: Tensor, k_scale: Tensor, v_scale: Tensor, k_newest: Tensor,
                  v_newest: Tensor, table: Tensor, rows: Optional[Tensor] = None):
-        if k_pages.dim() != 4 or k_pages.dtype != torch.uint8:
-            raise ValueError("k_pages: uint8 [pages, kv_heads, P, D] expected")
-        n, h, p, d = k_pages.shape
-        if p not in (16, 32, 64, 128) or d not in (32, 64, 128):
-            raise ValueError(f"page size {p}, head_dim {d}: a page size of 16, 32, 64 or 128 and a head_dim of 32, 64 or 128 expected")
-        if v_pages.dtype != torch.uint8 or v_pages.shape != (n, h, p // 4, d, 4):
-            raise ValueError("v_pages: uint8 [pages, kv_heads, P/4, D, 4] expected")
-        if k_scale.dtype != _f32 or v_scale.dtype != _f32 or k_scale.shape != (n, h) or v_scale.shape != (n, h):
-            raise ValueError("k_scale, v_scale: fp32 [pages, kv_heads] expected")
-        m, t16 = k_newest.shape[0], k_newest.dtype
-        if (t16 != torch.float16 and t16 != torch.bfloat16) or k_newest.shape != (m, 2, h, p, d):
-            raise ValueError("k_newest: fp16 or bf16 [rows, 2, kv_heads, P, D] expected")
-        if v_newest.dtype != t16 or v_newest.shape != (m, 2, h, p // 4, d, 4):
-            raise ValueError("v_newest: k_newest's type, [rows, 2, kv_heads, P/4, D, 4] expected")
-        if table.dtype != _i32 or table.dim() != 2:
-            raise ValueError("table: int32 [batch, blocks] expected")
-        b, w = table.shape
-        if not 1 <= b <= MAX_BATCH or w < 1 or n < 1 or m < 1:
-            raise ValueError(f"batch of 1 to {MAX_BATCH}, at least one page, row and block expected")
-        if rows is None and m < b:
-            raise ValueError("fewer rows of newest blocks than sequences")
-        self.tensors = ts = (k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows)
-        for t in ts:
-            if t is not None and not t.is_contiguous():
-                raise ValueError("cache tensors must be contiguous")
-        self.device = k_pages.device
-        self.index = self.device.index
-        _stream(self.index, *ts)
-        self.kv_heads, self.page_size, self.head_dim, self.dtype, self.batch = h, p, d, t16, b
-        self._c = rt.KvCache8(
-            k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_newest.data_ptr(),
-            v_newest.data_ptr(), table.data_ptr(), None if rows is None else _index(rows, b, "rows"), n, h, p, d, m, w, b,
-            t16 == torch.bfloat16)
+        self._c = _native().cache(k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows)
+        self.tensors = (k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows)
+
+    @property
+    def batch(self) -> int:
+        return self.tensors[6].shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.tensors[0].shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return self.tensors[0].shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self.tensors[0].shape[3]
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.tensors[4].dtype
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, table: Tensor,
@@ -130,51 +126,12 @@ class PagedKV8:
         strided): row cu[b] + i is token start[b] + i of sequence b (``cu`` int32 [batch + 1],
         ``start`` int32 [batch]).  ``cos`` / ``sin`` fp32 [positions, rot / 2]: the first ``rot``
         channels of a head turn in pairs (i, i + rot/2), or (2i, 2i + 1) if ``interleaved``."""
-        d, n = self.head_dim, qkv.shape[0]
-        width = (heads + 2 * self.kv_heads) * d
-        if heads <= 0 or heads % self.kv_heads:
-            raise ValueError(f"heads {heads}: a multiple of {self.kv_heads} expected")
-        if qkv.dim() != 2 or qkv.shape[1] != width or qkv.dtype != self.dtype:
-            raise ValueError(f"qkv: {self.dtype} [tokens, {width}] expected")
-        ld = width
-        if n > 1:
-            ld, dense = qkv.stride()
-            if dense != 1 or ld % 8 or ld < width:
-                raise ValueError("qkv: dense rows that start 16-byte aligned and do not overlap expected")
-        rot = turns = 0
-        if cos is not None or sin is not None:
-            if (cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != _f32 or
-                    sin.dtype != _f32 or not cos.is_contiguous() or not sin.is_contiguous()):
-                raise ValueError("cos, sin: both or neither, contiguous fp32 [positions, rot / 2] expected")
-            turns, rot = cos.shape[0], 2 * cos.shape[1]
-            if turns <= 0 or rot <= 0 or rot % 16 or rot > d:
-                raise ValueError(f"rotated channels {rot}: a multiple of 16 up to {d} expected")
-        if out is None:
-            out = torch.empty(n, heads, d, dtype=self.dtype, device=self.device)
-        elif out.shape != (n, heads, d) or out.dtype != self.dtype or not out.is_contiguous():
-            raise ValueError(f"out: contiguous {self.dtype} [{n}, {heads}, {d}] expected")
-        rc = rt.lib().b200_kv8_append(
-            self._c, qkv.data_ptr(), ld, out.data_ptr(), _index(cu, self.batch + 1, "cu"),
-            _index(start, self.batch, "start"), None if cos is None else cos.data_ptr(),
-            None if sin is None else sin.data_ptr(), rot, interleaved, turns, n, heads,
-            _stream(self.index, qkv, cu, start, cos, sin, out))
-        if rc:
-            rt.check(rc, "b200_kv8_append")
-        return out
+        return _done(_module.append(self._c, qkv, cu, start, heads, cos, sin, interleaved, out), "b200_kv8_append")
 
     def read(self, cu: Tensor, start: Tensor, lens: Tensor, *, total: int) -> Tuple[Tensor, Tensor]:
         """Keys and values as attention sees them, [total, kv_heads, D] each: row cu[b] + i is token
         start[b] + i of sequence b, of which lens[b] tokens are cached."""
-        if total < 0:
-            raise ValueError("total: the number of rows expected")
-        k = torch.empty(2, total, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.device)
-        v = k[1]
-        rc = rt.lib().b200_kv8_read(
-            self._c, _index(cu, self.batch + 1, "cu"), _index(start, self.batch, "start"), _index(lens, self.batch, "lens"),
-            k.data_ptr(), v.data_ptr(), total, _stream(self.index, cu, start, lens))
-        if rc:
-            rt.check(rc, "b200_kv8_read")
-        return k[0], v
+        return _done(_module.read(self._c, cu, start, lens, total), "b200_kv8_read")
 
     def attend(self, q: Tensor, cu: Tensor, lens: Tensor, *, max_q_len: int, scale: Optional[float] = None,
                out: Optional[Tensor] = None) -> Tensor:
@@ -183,40 +140,7 @@ class PagedKV8:
         Row cu[b] + i of ``q`` is the token at position lens[b] - n + i of sequence b (n = cu[b+1] -
         cu[b] <= ``max_q_len``), appended already; it sees the keys up to its own.  A row with no key
         gives zeros.  ``scale`` defaults to 1 / sqrt(D).  The same inputs give the same bits."""
-        d = self.head_dim
-        if q.dim() != 3 or q.shape[2] != d or q.dtype != self.dtype:
-            raise ValueError(f"q: {self.dtype} [tokens, heads, {d}] expected")
-        n, heads, _ = q.shape
-        if heads <= 0 or heads % self.kv_heads:
-            raise ValueError(f"heads {heads}: a multiple of {self.kv_heads} expected")
-        if max_q_len < 1 and n:
-            raise ValueError("max_q_len: at least 1 expected")
-        ld_q = self._rows(q, n, heads, d)
-        if out is None:
-            out = torch.empty(n, heads, d, dtype=self.dtype, device=self.device)
-            ld_out = heads * d
-        else:
-            if out.shape != q.shape or out.dtype != q.dtype:
-                raise ValueError("out: q's shape and type expected")
-            ld_out = self._rows(out, n, heads, d)
-        lib = rt.lib()
-        need = lib.b200_kv8_attention_workspace_bytes(self.batch, heads, self.kv_heads, d, max_q_len)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        rc = lib.b200_kv8_attention(
-            self._c, q.data_ptr(), ld_q, out.data_ptr(), ld_out, _index(cu, self.batch + 1, "cu"),
-            _index(lens, self.batch, "lens"), n, heads, max_q_len, 1 / math.sqrt(d) if scale is None else scale,
-            ws.data_ptr(), need, _stream(self.index, q, cu, lens, out))
-        if rc:
-            rt.check(rc, "b200_kv8_attention")
-        return out
-
-    @staticmethod
-    def _rows(t: Tensor, n: int, heads: int, d: int) -> int:
-        """The row stride of [tokens, heads, D], whose heads lie side by side."""
-        ld, per_head, dense = t.stride()
-        if dense != 1 or (heads > 1 and per_head != d) or (n > 1 and (ld % 8 or ld < heads * d)):
-            raise ValueError("q, out: the heads of a token must be dense, and rows start 16-byte aligned and not overlap")
-        return ld if n > 1 else heads * d
+        return _done(_module.attend(self._c, q, cu, lens, max_q_len, scale, out), "b200_kv8_attention")
 
 
 # ------------------------------------------------------------------ int8 linear
@@ -224,12 +148,12 @@ def quantize_weight(w: Tensor) -> Tuple[Tensor, Tensor]:
     """w [n, k] (fp16, bf16 or fp32) -> int8 codes [n, k rounded up to 16] and fp32 scale [n] (largest magnitude / 127)."""
     _need(w.dim() == 2 and w.dtype in _TYPES and w.shape[1] > 0, "w: fp16, bf16 or fp32 [n, k] expected")
     _need(w.stride(1) == 1 or w.shape[1] == 1, "w: rows must be dense")
-    stream = _stream(w.device.index, w)
+    _on_device(w)
     n, k = w.shape
     codes = torch.zeros(n, (k + 15) // 16 * 16, dtype=torch.int8, device=w.device)
     scale = torch.empty(n, device=w.device)
     rt.check(rt.lib().b200_quantize_rows_i8(w.data_ptr(), _TYPES[w.dtype], max(w.stride(0), k), codes.data_ptr(),
-                                            codes.shape[1], scale.data_ptr(), n, k, stream), "b200_quantize_rows_i8")
+                                            codes.shape[1], scale.data_ptr(), n, k, rt._stream()), "b200_quantize_rows_i8")
     return codes, scale
 
 
@@ -242,49 +166,7 @@ def linear_int8(x: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = 
     of 16, at least k (``quantize_weight``); ``w_scale`` and ``bias`` fp32 [n].  With ``gelu`` the
     exact GELU follows.  ``resid`` fp32 [m, n] is added last: the result is fp32, and ``out`` may be
     ``resid`` itself.  Without it the result has ``out_dtype`` (default: x's type)."""
-    xt = _TYPES.get(x.dtype)
-    if xt is None or x.dim() != 2:
-        raise ValueError("x: fp16, bf16 or fp32 [m, k] expected")
-    m, k = x.shape
-    ld_x, dense = x.stride()
-    if k < 1 or (dense != 1 and k > 1) or (ld_x < k and m > 1):
-        raise ValueError("x: dense rows that do not overlap expected")
-    if w.dim() != 2 or w.dtype != torch.int8 or not k <= w.shape[1] < k + 16 or w.stride(1) != 1 or w.stride(0) % 16:
-        raise ValueError(f"w: int8 [n, {(k + 15) // 16 * 16}] with a row pitch that is a multiple of 16 expected")
-    n = w.shape[0]
-    if w_scale.dtype != _f32 or w_scale.shape != (n,) or not w_scale.is_contiguous():
-        raise ValueError(f"w_scale: contiguous fp32 [{n}] expected")
-    if bias is not None and (bias.dtype != _f32 or bias.shape != (n,) or not bias.is_contiguous()):
-        raise ValueError(f"bias: contiguous fp32 [{n}] expected")
-    dt = x.dtype if out_dtype is None else out_dtype
-    ld_r = n
-    if resid is not None:
-        if gelu or out_dtype not in (None, _f32):
-            raise ValueError("with resid the result is fp32, and there is no GELU")
-        if resid.dtype != _f32 or resid.shape != (m, n) or (resid.stride(1) != 1 and n > 1):
-            raise ValueError(f"resid: fp32 [{m}, {n}] expected")
-        dt, ld_r = _f32, max(resid.stride(0), n)
-    ot = _TYPES.get(dt)
-    if ot is None:
-        raise ValueError("out_dtype: fp16, bf16 or fp32 expected")
-    ld_out = n
-    if out is None:
-        out = torch.empty(m, n, dtype=dt, device=x.device)
-    else:
-        if out.shape != (m, n) or out.dtype != dt or (out.stride(1) != 1 and n > 1) or (out.stride(0) < n and m > 1):
-            raise ValueError(f"out: {dt} [{m}, {n}] with dense rows expected")
-        ld_out = max(out.stride(0), n)
-    stream = _stream(x.device.index, x, w, w_scale, bias, resid, out)
-    lib = rt.lib()
-    need = lib.b200_linear_i8_workspace_bytes(m, k)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    a = rt.LinearI8Args(x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                        None if resid is None else resid.data_ptr(), out.data_ptr(), max(ld_x, k), w.stride(0), ld_r,
-                        ld_out, m, n, k, xt, ot, gelu, ws.data_ptr(), need)
-    rc = lib.b200_linear_i8(a, stream)
-    if rc:
-        rt.check(rc, "b200_linear_i8")
-    return out
+    return _done(_native().linear(x, w, w_scale, bias, gelu, resid, out_dtype, out), "b200_linear_i8")
 
 
 # ------------------------------------------------------------------ a block stack served in 8 bits
@@ -359,7 +241,7 @@ class Int8Decoder:
         total = sum(counts)
         _need(x.shape == (total, cfg.d_model) and x.dtype == torch.float32 and x.is_contiguous(),
               f"x: contiguous fp32 [{total}, {cfg.d_model}] expected")
-        _stream(self.dev.index, x)
+        _on_device(x)
         _need(all(self.lens[s] + c <= self.table.shape[1] * p for s, c in zip(seqs, counts)), "a sequence over max_tokens")
         if total == 0:
             return torch.empty_like(x)
