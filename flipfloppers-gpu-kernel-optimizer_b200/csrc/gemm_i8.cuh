@@ -511,4 +511,197 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * GEMM2_I8_E
   }
 }
 
+// Few rows (M <= 64): one kernel that quantizes and multiplies.  The weight is what has to be read, so w's rows fill
+// the 128 rows of the tcgen05 step and x's rows its N = 16 .. 64 columns, and a cluster of CTAs splits K:
+//   - each CTA's slices of w (128 rows x 128 bytes, at most LIN_SLICES) come by TMA while
+//   - its warps find the rows' maxima over the CTA's part of K, exchange them in the cluster, and write the codes of
+//     x in SWIZZLE_128B order;
+//   - the partial int32 sums (exact, so any order gives the same bits) go to shared memory, and each CTA adds and
+//     finishes a share of the rows through distributed shared memory.
+// Latency-bound.  Against the quantizer and the 128x128 kernel one after the other: 1x1024x4096 GELU 8.3 -> 5.4 us,
+// 64x4096x1024 residual 18.9 -> 10.6 us (device time in a CUDA graph; 8 warps a CTA up to 16 rows, where 16 take
+// 6.1 us, and 16 above, where 8 take 13.9 us: the quantization's instructions).
+constexpr int LIN_ROWS = 64, LIN_SLICES = 8, LIN_MAX_CLUSTER = 8, LIN_MAX_WARPS = 16;
+
+struct LinSmallParams {
+  GemmI8Params g;      // (g.sx unused)
+  const void* x;
+  long long ldx;
+  int vec, out_type, epi;
+  int pad, slices, cluster;  // rows of x rounded up to 16, K slices a CTA, CTAs a cluster
+};
+struct LinSmallSmem {
+  static constexpr int W_SLICE = 128 * 128;
+  int x_off, meta_off, total;
+  __host__ __device__ LinSmallSmem(int pad, int slices) {
+    const int w = slices * W_SLICE, acc = pad * 128 * 4;
+    x_off = w > acc ? w : (acc + 1023) / 1024 * 1024;
+    meta_off = x_off + slices * pad * 128;
+    total = meta_off + 2 * LIN_ROWS * 4 + 64 + 1024;
+  }
+};
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(32 * LIN_MAX_WARPS, 1) k_lin_small(const __grid_constant__ CUtensorMap tmW, const LinSmallParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_align1024(smem_raw);
+  const LinSmallSmem L(p.pad, p.slices);
+  unsigned* tops = reinterpret_cast<unsigned*>(smem + L.meta_off);
+  float* sx = reinterpret_cast<float*>(tops + LIN_ROWS);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sx + LIN_ROWS);
+  uint64_t* done = full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  const int rank = static_cast<int>(cluster_ctarank()), n0 = static_cast<int>(blockIdx.x) / p.cluster * 128;
+  const int M = p.g.M, K = p.g.K;
+  const int s0 = rank * p.slices, ns = max(0, min(p.slices, (K + 127) / 128 - s0));  // this CTA's slices
+  const int k0 = s0 * 128, k1 = min(K, k0 + ns * 128);
+  const uint32_t cols = p.pad <= 32 ? 32 : 64;
+  if (tid == 0) {
+    mbar_init(full, 1);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_sync();
+  if (tid == 0 && ns > 0) {
+    mbar_arrive_expect_tx(full, ns * LinSmallSmem::W_SLICE);
+    for (int s = 0; s < ns; ++s) tma_load_2d(smem + s * LinSmallSmem::W_SLICE, &tmW, full, (s0 + s) * 128, n0);
+  }
+  __syncwarp();
+  // the rows' maxima over this CTA's part of K: four rows a warp side by side, 16 values a lane of each
+  for (int r0 = warp; r0 < M; r0 += 4 * warps) {
+    unsigned top[4] = {0, 0, 0, 0};
+    for (int k = k0 + lane * 16; k < k1; k += 512) {
+      float v[4][16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + warps * i < M) load_row16<DT>(p.x, (r0 + warps * i) * p.ldx, k, k1, p.vec && k + 16 <= k1, v[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + warps * i < M)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top[i] = max(top[i], __float_as_uint(v[i][j]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+      if (lane == 0 && r0 + warps * i < M) tops[r0 + warps * i] = top[i];
+    }
+  }
+  __syncthreads();
+  cluster_sync_all();
+  if (tid < M) {
+    unsigned each[LIN_MAX_CLUSTER], top = 0;
+#pragma unroll
+    for (int c = 0; c < LIN_MAX_CLUSTER; ++c) each[c] = ld_cluster_u32(mapa_shared(smem_u32(tops + tid), c & (p.cluster - 1)));
+#pragma unroll
+    for (int c = 0; c < LIN_MAX_CLUSTER; ++c) top = max(top, each[c]);
+    sx[tid] = top < 0x7f800000u ? __fmul_rn(__uint_as_float(top), 1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+  }
+  __syncthreads();
+  for (int r0 = warp; r0 < M; r0 += 4 * warps)
+    for (int k = lane * 16; k < ns * 128; k += 512) {
+      float v[4][16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + warps * i < M) load_row16<DT>(p.x, (r0 + warps * i) * p.ldx, k0 + k, k1, p.vec && k0 + k + 16 <= k1, v[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + warps * i;
+        if (r >= M) break;
+        const float s = sx[r], inv = __fdiv_rn(1.f, s);
+        const bool small = s < 1e-30f;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (s > 0.f) {  // false: a row of zeros, or NaN
+          w.x = quantize4(v[i][0], v[i][1], v[i][2], v[i][3], s, inv, small);
+          w.y = quantize4(v[i][4], v[i][5], v[i][6], v[i][7], s, inv, small);
+          w.z = quantize4(v[i][8], v[i][9], v[i][10], v[i][11], s, inv, small);
+          w.w = quantize4(v[i][12], v[i][13], v[i][14], v[i][15], s, inv, small);
+        }
+        *reinterpret_cast<uint4*>(smem + L.x_off + (k >> 7) * p.pad * 128 + sw128_off(r, (k >> 4) & 7)) = w;
+      }
+    }
+  fence_proxy_async_smem();
+  __syncthreads();
+  bool ok = true;
+  if (ns > 0) {
+    if (warp == 1 && lane == 0) {
+      if (mbar_wait(full, 0, abort_flag, DERR_WAIT_TMA)) {
+        tc_fence_after();
+        const uint32_t idesc = make_idesc_i8(128, p.pad);
+        for (int s = 0; s < ns; ++s) {
+          const uint32_t a = smem_u32(smem + s * LinSmallSmem::W_SLICE), b = smem_u32(smem + L.x_off + s * p.pad * 128);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_i8_ss(tmem, make_sdesc(a + kk * 32, 16, 1024, UMMA_SW128), make_sdesc(b + kk * 32, 16, 1024, UMMA_SW128),
+                       idesc, (s | kk) != 0 ? 1u : 0u);
+        }
+        tc_commit(done);
+      } else {
+        mbar_wait_drain(full, 0);
+      }
+    }
+    __syncwarp();
+    ok = mbar_wait_warp(done, 0, abort_flag, DERR_WAIT_MMA);
+    if (ok) tc_fence_after();
+  }
+  // the sums, [row of x][column], over the slices of w (which every product has read)
+  int* acc = reinterpret_cast<int*>(smem);
+  __syncthreads();
+  for (int c = (warp >> 2) * 16; c < p.pad; c += warps * 4) {
+    float v[16];
+    if (ns > 0 && ok) {
+      tmem_ld16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[(c + j) * 128 + (warp & 3) * 32 + lane] = __float_as_int(v[j]);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  const int col = n0 + (tid & 127);
+  if (col < p.g.N) {
+    const float sw = __ldg(p.g.sw + col), bias = p.g.bias ? __ldg(p.g.bias + col) : 0.f;
+#pragma unroll 4
+    for (int m = rank + p.cluster * (tid >> 7); m < M; m += (warps >> 2) * p.cluster) {
+      const uint32_t at = smem_u32(acc + m * 128 + (tid & 127));
+      int each[LIN_MAX_CLUSTER], sum = 0;  // one round trip for all
+#pragma unroll
+      for (int c = 0; c < LIN_MAX_CLUSTER; ++c) each[c] = c < p.cluster ? static_cast<int>(ld_cluster_u32(mapa_shared(at, c))) : 0;
+#pragma unroll
+      for (int c = 0; c < LIN_MAX_CLUSTER; ++c) sum += each[c];
+      float y = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(sum), sx[m]), sw), bias);
+      if (p.epi == I8_GELU) y = gelu_as(y);
+      if (p.epi == I8_RESID) y = __fadd_rn(__ldg(p.g.resid + m * p.g.ld_resid + col), y);
+      const long long to = m * p.g.ld_out + col;
+      if (p.out_type == DT_F32) static_cast<float*>(p.g.out)[to] = y;
+      else static_cast<uint16_t*>(p.g.out)[to] = static_cast<uint16_t>(f_to_h16(y, p.out_type == DT_BF16));
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
 }  // namespace b200

@@ -336,7 +336,8 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out = at::empty({m, N}, x.options().dtype(type));
     }
     const size_t bytes = b200_linear_i8_workspace_bytes(static_cast<int>(m), static_cast<int>(k));
-    const at::Tensor space = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+    at::Tensor space;
+    if (bytes) space = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
     B200LinearI8Args p{};
     p.x = x.data_ptr();
     p.w = w.data_ptr();
@@ -354,7 +355,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.x_type = xt;
     p.out_type = ot;
     p.gelu = gelu;
-    p.workspace = space.data_ptr();
+    p.workspace = bytes ? space.data_ptr() : nullptr;
     p.workspace_bytes = bytes;
     const int rc = b200_linear_i8(&p, st);
     return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));

@@ -203,8 +203,10 @@ int make_map_i8(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, 
 
 long long i8_pitch(int K) { return (static_cast<long long>(K) + 15) / 16 * 16; }
 
+bool lin_small_fits(int m, int k);
+
 size_t linear_i8_workspace(int M, int K) {
-  if (M <= 0 || K <= 0) return 0;
+  if (M <= 0 || K <= 0 || lin_small_fits(M, K)) return 0;
   return static_cast<size_t>(M) * i8_pitch(K) + static_cast<size_t>(M) * sizeof(float);
 }
 
@@ -259,6 +261,37 @@ int launch_gemm_i8(const GemmI8Params& p, const CUtensorMap& ta, const void* w, 
   return launch_status();
 }
 
+// The one-kernel form for few rows: CTAs of a cluster split K, at most LIN_SLICES slices of 128 each.
+bool lin_small_fits(int m, int k) { return m <= LIN_ROWS && k <= LIN_MAX_CLUSTER * LIN_SLICES * 128; }
+
+int launch_lin_small(const GemmI8Params& g, const B200LinearI8Args* a, cudaStream_t st) {
+  LinSmallParams p{};
+  p.g = g;
+  p.x = a->x;
+  p.ldx = a->ld_x;
+  p.vec = al16(a->x) && a->ld_x % (a->x_type == DT_F32 ? 4 : 8) == 0;
+  p.out_type = a->out_type;
+  p.epi = a->resid ? I8_RESID : a->gelu ? I8_GELU : I8_BIAS;
+  p.pad = (a->m + 15) / 16 * 16;
+  // as many CTAs a cluster as fill the SMs once, at least those that hold K
+  const int tiles = (a->n + 127) / 128, all = (a->k + 127) / 128;
+  p.cluster = 1;
+  while (p.cluster < LIN_MAX_CLUSTER && p.cluster < all &&
+         ((all + p.cluster - 1) / p.cluster > LIN_SLICES || 2LL * p.cluster * tiles <= num_sms()))
+    p.cluster *= 2;
+  p.slices = (all + p.cluster - 1) / p.cluster;
+  if (static_cast<long long>(tiles) * p.cluster > 0x7fffffffLL) return B200_ERR_TILE;
+  CUtensorMap tw;
+  if (int rc = make_map_i8(&tw, a->w, a->n, a->k, a->ld_w, 128)) return rc;
+  auto kern = a->x_type == DT_F16 ? k_lin_small<DT_F16> : a->x_type == DT_BF16 ? k_lin_small<DT_BF16> : k_lin_small<DT_F32>;
+  const int smem = LinSmallSmem(p.pad, p.slices).total;
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), LinSmallSmem(LIN_ROWS, LIN_SLICES).total)) return rc;
+  launch_kernel_cluster(kern, dim3(static_cast<unsigned>(tiles * p.cluster)), dim3(p.pad == 16 ? 256 : 32 * LIN_MAX_WARPS),
+                        smem, st,
+                        static_cast<unsigned>(p.cluster), tw, p);
+  return launch_status();
+}
+
 int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   if (!a || a->m < 0 || a->n <= 0 || a->k <= 0) return B200_ERR_ARG;
   if (a->x_type < 0 || a->x_type > 2 || a->out_type < 0 || a->out_type > 2) return B200_ERR_CONFIG;
@@ -269,26 +302,30 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   if (a->ld_w % 16 || !al16(a->w)) return B200_ERR_ALIGN;
   // the sums are int32: |sum| <= 127 * 127 * k
   if (a->k > 133000) return B200_ERR_TILE;
-  if (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k)) return B200_ERR_WORKSPACE;
-  if (!al16(a->workspace)) return B200_ERR_ALIGN;
+  const bool few = lin_small_fits(a->m, a->k);
+  if (!few) {
+    if (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k)) return B200_ERR_WORKSPACE;
+    if (!al16(a->workspace)) return B200_ERR_ALIGN;
+  }
   if (int rc = check_arch()) return rc;
-  const long long pitch = i8_pitch(a->k);
-  int8_t* codes = static_cast<int8_t*>(a->workspace);
-  float* sx = reinterpret_cast<float*>(codes + static_cast<size_t>(a->m) * pitch);
-  if (int rc = quantize_rows_impl(a->x, a->x_type, a->ld_x, codes, pitch, sx, a->m, a->k, st)) return rc;
-  CUtensorMap ta;
-  if (int rc = make_map_i8(&ta, codes, a->m, a->k, pitch, 128)) return rc;
   GemmI8Params p{};
   p.M = a->m;
   p.N = a->n;
   p.K = a->k;
-  p.sx = sx;
   p.sw = a->w_scale;
   p.bias = a->bias;
   p.resid = a->resid;
   p.ld_resid = a->ld_resid;
   p.out = a->out;
   p.ld_out = a->ld_out;
+  if (few) return launch_lin_small(p, a, st);
+  const long long pitch = i8_pitch(a->k);
+  int8_t* codes = static_cast<int8_t*>(a->workspace);
+  float* sx = reinterpret_cast<float*>(codes + static_cast<size_t>(a->m) * pitch);
+  if (int rc = quantize_rows_impl(a->x, a->x_type, a->ld_x, codes, pitch, sx, a->m, a->k, st)) return rc;
+  CUtensorMap ta;
+  if (int rc = make_map_i8(&ta, codes, a->m, a->k, pitch, 128)) return rc;
+  p.sx = sx;
   p.tma_out = al16(a->out) && a->ld_out * (a->out_type == DT_F32 ? 4 : 2) % 16 == 0;
   auto go = [&](auto f) { return f(p, ta, a->w, a->ld_w, st); };
   if (a->resid) return go(launch_gemm_i8<DT_F32, I8_RESID>);

@@ -384,7 +384,7 @@ typedef struct {
   long long ld_x, ld_w, ld_resid, ld_out;
   int m, n, k;
   int x_type, out_type, gelu;
-  void* workspace;        /* >= b200_linear_i8_workspace_bytes(m, k), 16-byte aligned */
+  void* workspace;        /* >= b200_linear_i8_workspace_bytes(m, k) (0 for few rows), 16-byte aligned */
   size_t workspace_bytes;
 } B200LinearI8Args;
 /* x [m, k] of x_type -> int8 codes [m, k] (row pitch ld_codes bytes) and scale [m]: the

@@ -95,7 +95,8 @@ def test_linear_checks(pkg):
     assert linear(ld_w=72) == -5
     assert linear(w=4104) == -5
     assert linear(k=200000, ld_x=200000, ld_w=200000) == -2  # sums past int32
-    assert linear(workspace_bytes=8) == -12
+    assert linear(m=100, workspace_bytes=8) == -12
+    assert lib.b200_linear_i8_workspace_bytes(64, 64) == 0 < lib.b200_linear_i8_workspace_bytes(65, 64)  # few rows need none
     assert lib.b200_quantize_rows_i8(4096, 5, 8, 4096, 16, 64, 1, 8, None) == -1
     assert lib.b200_quantize_rows_i8(4096, 0, 7, 4096, 16, 64, 1, 8, None) == -9
     assert lib.b200_quantize_rows_i8(4096, 0, 8, 4096, 16, 64, 0, 8, None) == 0
