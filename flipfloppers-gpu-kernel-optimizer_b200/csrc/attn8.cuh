@@ -29,6 +29,8 @@
 namespace b200 {
 
 constexpr int ATTN8_CHUNK = 32;   // tokens
+// Weights are kept times 2^14 (at most 16384), so that fp16 has eleven bits for those down to 2^-28 of the largest.
+constexpr float ATTN8_LIFT = 14.f;
 constexpr int ATTN8_MAX_BATCH = 2048;
 
 struct Attn8Params {
@@ -337,8 +339,9 @@ struct Attn8Warp {
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
         const float now = fmaxf(m[n][e], x);
-        const float ref = now == -INFINITY ? 0.f : now;  // no key seen yet: every weight is 0
-        alpha[n][e] = fast_exp2(m[n][e] - ref);
+        const float top = now == -INFINITY ? 0.f : now;  // no key seen yet: every weight is 0
+        const float ref = top - ATTN8_LIFT;
+        alpha[n][e] = fast_exp2(m[n][e] - top);
         moved |= now != m[n][e];
         m[n][e] = now;
         float sum = 0.f;

@@ -1,0 +1,573 @@
+// Attention over the 8-bit paged cache for many rows (chunks of prompts): the same
+// operator as attn8.cuh on tcgen05.  A CTA takes 256 rows of one key head (query heads
+// of its group times new tokens) as two 128-row tiles and walks the keys in tiles of
+// 128:
+//   warps 1-3    bring the codes from the pages to registers a tile ahead, widen them to
+//                fp16 whole numbers (exact) and store K and V in the swizzled layouts the
+//                MMAs read, once for both row tiles; Q likewise at the start of an item;
+//   warp 0       issues S = Q K^T and O += P V for the two tiles in turn;
+//   warps 4-11   softmax, a warpgroup a row tile, one row a thread; P overwrites S in
+//                tensor memory.  While one tile is in its exponentials the tensor core
+//                works for the other.
+// Scales: with w = s + log2(V scale), P = 2^(w - max w + 14) carries a key's V scale (P <= 2^14,
+// and O needs no scale of its own), and the softmax's sum takes P / (V scale).  K's scale
+// multiplies the score.  A block of zeros counts as scale 2^-100.  The newest block's
+// 16-bit values are brought into fp16 by a power of two for each token (exact to 2^-24
+// of the token's largest value); a token whose V has an infinity or NaN gives NaN to the
+// rows that see it and nothing to the others.
+// Bound: the exponentials (16 a clock and SM), 2048 clocks for two 128x128 tiles.
+#pragma once
+
+#include "attn8.cuh"
+
+namespace b200 {
+
+template <int D>
+struct Attn8TileCfg {
+  static constexpr int BN = 128, ST = 2, ROWS = 256, THREADS = 384, CONV = 96;
+  static constexpr int ATOM = D >= 64 ? 64 : D;      // channels a swizzle row
+  static constexpr int ROWB = ATOM * 2;              // its bytes
+  static constexpr uint32_t SWZ = ATOM == 64 ? UMMA_SW128 : UMMA_SW64;
+  static constexpr int NBOX = D / ATOM;
+  static constexpr int Q_BYTES = 128 * D * 2;        // one row tile
+  static constexpr int KV_BYTES = BN * D * 2;
+  static constexpr int OFF_KV = 2 * Q_BYTES;         // stage s: K, then V
+  static constexpr int OFF_KEY = OFF_KV + ST * 2 * KV_BYTES;        // [ST][3][BN]: K factor, log2 V scale, 1 / V scale
+  static constexpr int OFF_QF = OFF_KEY + ST * 3 * BN * 4;          // [2][ROWS] row factors, by item parity
+  static constexpr int OFF_BAR = OFF_QF + 2 * ROWS * 4;
+  static constexpr int TOTAL = OFF_BAR + 256;        // + line + alignment
+  // tensor memory: S/P of the tiles at 0 and 128, O at 256 and 256 + D
+  static constexpr uint32_t TM_O = 256;
+};
+
+struct Attn8Item {
+  int b, head, row0;     // first of its 256 rows
+  int t0, q_len, len, full, nkt;
+  int rows;              // of the sequence and key head
+};
+__device__ __forceinline__ int attn8_limit(const Attn8Item& it, int row, int group) {
+  const int i = row / group;
+  return i < it.q_len ? max(0, it.len - it.q_len + i + 1) : 0;
+}
+// item `at` of the line (longest first within a sequence)
+__device__ __forceinline__ Attn8Item attn8_item(const Attn8Params& p, const int* line, int at) {
+  Attn8Item it;
+  int lo = 0, hi = p.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (line[mid] <= at) lo = mid; else hi = mid;
+  }
+  it.b = lo;
+  attn8_sequence(p, lo, it.t0, it.q_len, it.len);
+  const int group = p.heads / p.c.kv_heads;
+  it.rows = it.q_len * group;
+  const int tiles = (it.rows + 255) / 256, i = at - line[lo];
+  it.head = i % p.c.kv_heads;
+  it.row0 = (tiles - 1 - i / p.c.kv_heads) * 256;
+  it.full = it.len & ~(p.c.page - 1);
+  it.nkt = (attn8_limit(it, min(it.rows, it.row0 + 256) - 1, group) + 127) / 128;
+  return it;
+}
+
+template <int D>
+__device__ __forceinline__ uint32_t attn8_off(int rows, int row, int d) {  // of channel d in a [rows, D] operand tile
+  using C = Attn8TileCfg<D>;
+  const int box = d / C::ATOM, ch = (d % C::ATOM) >> 3;
+  const uint32_t sw = C::ATOM == 64 ? (row & 7) : ((row >> 1) & 3);
+  return box * rows * C::ROWB + row * C::ROWB + ((ch ^ sw) << 4) + (d & 7) * 2;
+}
+// 2^e as a float, and the exponent that brings the largest of 16-bit values (their magnitude bits) to [2^10, 2^11)
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ int exponent_down(unsigned top, int bf16) {
+  const float v = h16_to_f(top, bf16);
+  if (!(v > 0.f && v < INFINITY)) return 0;
+  return max(-126, min(126, static_cast<int>(__float_as_uint(v) >> 23) - 127 - 10));
+}
+__device__ __forceinline__ uint4 scale8(uint4 w, int bf16, float f) {  // eight 16-bit values times f, as fp16
+  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = pack_half2(h16_to_f(u[i] & 0xffffu, bf16) * f, h16_to_f(u[i] >> 16, bf16) * f);
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ unsigned top2(unsigned top, uint32_t w) { return __vmaxu2(top, w & 0x7fff7fffu); }
+
+// One softmax step of a row: raw scores s (in registers), key factors in shared memory.
+template <bool EACH>  // EACH: factors differ key by key (the newest block's tile), else every 16 keys
+__device__ __forceinline__ void attn8_weights(float (&s)[128], const float* key, float qf, int k0, int lim, bool masked, float& m,
+                                              float& l, float& alpha) {
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    if constexpr (EACH) {
+#pragma unroll
+      for (int c = 16 * g; c < 16 * g + 16; c += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(key + c), v = *reinterpret_cast<const float4*>(key + 128 + c);
+        s[c] = fmaf(s[c], f.x * qf, v.x);
+        s[c + 1] = fmaf(s[c + 1], f.y * qf, v.y);
+        s[c + 2] = fmaf(s[c + 2], f.z * qf, v.z);
+        s[c + 3] = fmaf(s[c + 3], f.w * qf, v.w);
+      }
+    } else {
+      const float f = key[16 * g] * qf, v = key[128 + 16 * g];
+      const uint64_t f2 = f2pk(f, f), v2 = f2pk(v, v);
+#pragma unroll
+      for (int c = 16 * g; c < 16 * g + 16; c += 2) f2upk(f2fma(f2pk(s[c], s[c + 1]), f2, v2), s[c], s[c + 1]);
+    }
+  }
+  if (masked) {
+#pragma unroll
+    for (int c = 0; c < 128; ++c)
+      if (k0 + c >= lim) s[c] = -INFINITY;
+  }
+  const float now = fmaxf(m, row_max<128>(s));
+  const float most = now == -INFINITY ? 0.f : now, ref = most - ATTN8_LIFT;
+  alpha = fast_exp2(m - most);
+  m = now;
+  const uint64_t nr = f2pk(-ref, -ref);
+  float sum = 0.f;
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    if constexpr (EACH) {
+#pragma unroll
+      for (int c = 16 * g; c < 16 * g + 16; c += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(key + 256 + c);
+        s[c] = fast_exp2(s[c] - ref);
+        s[c + 1] = fast_exp2(s[c + 1] - ref);
+        s[c + 2] = fast_exp2(s[c + 2] - ref);
+        s[c + 3] = fast_exp2(s[c + 3] - ref);
+        sum = fmaf(s[c], v.x, fmaf(s[c + 1], v.y, fmaf(s[c + 2], v.z, fmaf(s[c + 3], v.w, sum))));
+      }
+    } else {
+      uint64_t a0 = f2pk(0.f, 0.f), a1 = a0;
+#pragma unroll
+      for (int c = 16 * g; c < 16 * g + 16; c += 4) {
+        float x, y, z, w;
+        f2upk(f2add(f2pk(s[c], s[c + 1]), nr), x, y);
+        f2upk(f2add(f2pk(s[c + 2], s[c + 3]), nr), z, w);
+        s[c] = fast_exp2(x); s[c + 1] = fast_exp2(y); s[c + 2] = fast_exp2(z); s[c + 3] = fast_exp2(w);
+        a0 = f2add(a0, f2pk(s[c], s[c + 1]));
+        a1 = f2add(a1, f2pk(s[c + 2], s[c + 3]));
+      }
+      float x, y;
+      f2upk(f2add(a0, a1), x, y);
+      sum = fmaf(x + y, key[256 + 16 * g], sum);
+    }
+  }
+  l = l * alpha + sum;
+}
+
+template <int D>
+__global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(const Attn8Params p) {
+  using C = Attn8TileCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int tot[C::THREADS / 32];
+  uint8_t* smem = smem_align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars;        // the converting threads
+  uint64_t* q_free = bars + 1;    // the item's last S MMA has read Q
+  uint64_t* kv_full = bars + 2;   // [ST] the converting threads
+  uint64_t* kv_empty = bars + 4;  // [ST] both tiles' PV have read the stage
+  uint64_t* s_full = bars + 6;    // [2]
+  uint64_t* p_full = bars + 8;    // [2] 128 softmax threads
+  uint64_t* o_done = bars + 10;   // [2]
+  uint64_t* drain = bars + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* line = reinterpret_cast<int*>(smem + C::TOTAL);  // [batch + 1] first item of each sequence
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = p.heads / p.c.kv_heads;
+  if (tid == 0) {
+    mbar_init(q_full, C::CONV);
+    mbar_init(q_free, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&kv_full[i], C::CONV);
+      mbar_init(&kv_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  griddep_sync();
+  int items = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += C::THREADS) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < p.batch) {
+      int t0, q_len, len;
+      attn8_sequence(p, b, t0, q_len, len);
+      n = p.c.kv_heads * ((q_len * group + 255) / 256);
+    }
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 31) tot[warp] = sum;
+    __syncthreads();
+    int before = items;
+    for (int i = 0; i < C::THREADS / 32; ++i) {
+      if (i < warp) before += tot[i];
+      items += tot[i];
+    }
+    if (b < p.batch) line[b] = before + sum - n;
+    __syncthreads();
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int G = gridDim.x;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc_f16(128, 128, false), idesc_o = make_idesc_f16(128, D, true);
+      auto issue_s = [&](int x, int st) {
+        const uint32_t q = smem_u32(smem + x * C::Q_BYTES), k = smem_u32(smem + C::OFF_KV + st * 2 * C::KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int box = kk * 16 / C::ATOM;
+          const uint32_t in = kk * 16 % C::ATOM * 2;
+          umma_f16_ss(tmem + x * 128, make_sdesc(q + box * 128 * C::ROWB + in, 16, 8 * C::ROWB, C::SWZ),
+                      make_sdesc(k + box * 128 * C::ROWB + in, 16, 8 * C::ROWB, C::SWZ), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[x]);
+      };
+      auto issue_pv = [&](int x, int st, bool first) {
+        const uint32_t v = smem_u32(smem + C::OFF_KV + st * 2 * C::KV_BYTES + C::KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_f16_ts(tmem + C::TM_O + x * D, tmem + x * 128 + 8 * kk,
+                      make_sdesc(v + kk * 16 * C::ROWB, 128 * C::ROWB, 8 * C::ROWB, C::SWZ), idesc_o, first && kk == 0 ? 0u : 1u);
+        tc_commit(&o_done[x]);
+      };
+      int g = 0, k = 0;  // key tiles and items so far
+      bool ok = true;
+      for (int at = blockIdx.x; ok && at < items; at += G) {
+        const int nkt = attn8_item(p, line, at).nkt;
+        if (nkt == 0) continue;
+        if (!mbar_wait(q_full, k & 1, abort_flag, DERR_WAIT_SLOT)) break;
+        for (int j = 0; ok && j <= nkt; ++j) {
+          // PV of tile j - 1 and S of tile j, for each row tile; S overwrites the P that the PV has read
+          if (j < nkt) {
+            ok = mbar_wait(&kv_full[(g + j) % C::ST], (g + j) / C::ST & 1, abort_flag, DERR_WAIT_SLOT);
+            if (!ok) break;
+          }
+          for (int x = 0; ok && x < 2; ++x) {
+            if (j > 0) {
+              ok = mbar_wait(&p_full[x], (g + j - 1) & 1, abort_flag, DERR_WAIT_SOFTMAX);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(x, (g + j - 1) % C::ST, j == 1);
+              if (x == 1) tc_commit(&kv_empty[(g + j - 1) % C::ST]);
+              if (j < nkt) {
+                ok = mbar_wait(&o_done[x], (g + j - 1) & 1, abort_flag, DERR_WAIT_MMA);
+                if (!ok) break;
+              }
+            } else if (g > 0) {
+              ok = mbar_wait(&o_done[x], (g - 1) & 1, abort_flag, DERR_WAIT_MMA);
+              if (!ok) break;
+            }
+            if (j < nkt) {
+              tc_fence_after();
+              issue_s(x, (g + j) % C::ST);
+              if (x == 1 && j == nkt - 1) tc_commit(q_free);
+            }
+          }
+        }
+        g += nkt;
+        ++k;
+      }
+      if (*abort_flag) {
+        tc_commit(drain);
+        mbar_wait_drain(drain, 0);
+      }
+    }
+  } else if (warp < 4) {
+    const int i = tid - 32, P = p.c.page, psh = p.c.page_shift, cw = warp - 1;
+    constexpr int NC = D / 16, ALL = 128 * NC;                 // 16-byte chunks of K, and of V: of a token, of a tile,
+    constexpr int MINE = (ALL + C::CONV - 1) / C::CONV;        // of a thread
+    uint4 kr[MINE], vr[MINE];
+    int g = 0, k = 0;
+    bool ok = true;
+    for (int at = blockIdx.x; ok && at < items; at += G) {
+      const Attn8Item it = attn8_item(p, line, at);
+      if (it.nkt == 0) continue;
+      // page of block `blk` of the sequence (those in full blocks)
+      auto page_of = [&](int blk) -> size_t {
+        int id = __ldg(p.c.table + static_cast<size_t>(it.b) * p.c.table_width + blk);
+        if (id < 0 || id >= p.c.num_pages) {
+          record_error(DERR_KV_RANGE);
+          id = 0;
+        }
+        return static_cast<size_t>(id) * p.c.kv_heads + it.head;
+      };
+      // a tile's pages, one a lane, a tile ahead of its codes
+      auto tile_page = [&](int j) {
+        const int blk = (j << (7 - psh)) + lane;
+        return lane < (128 >> psh) && blk < (it.full >> psh) ? static_cast<uint32_t>(page_of(blk)) : 0u;
+      };
+      auto fetch = [&](int j, uint32_t pages) {
+        const int limit = it.full - 128 * j;  // keys of the tile in full blocks
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+          const int c = min(i + C::CONV * u, ALL - 1), kt = c / NC, vt = c / (D / 4) * 4;
+          const size_t ka = static_cast<size_t>(__shfl_sync(0xffffffffu, pages, kt >> psh)) * P * D + (kt & (P - 1)) * D + c % NC * 16;
+          const size_t va = static_cast<size_t>(__shfl_sync(0xffffffffu, pages, vt >> psh)) * P * D + (vt & (P - 1)) * D + c % (D / 4) * 16;
+          kr[u] = kt < limit ? __ldg(reinterpret_cast<const uint4*>(p.c.k_pages + ka)) : make_uint4(0, 0, 0, 0);
+          vr[u] = vt < limit ? __ldg(reinterpret_cast<const uint4*>(p.c.v_pages + va)) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      uint32_t pages = tile_page(0);
+      fetch(0, pages);
+      // Q: rows in turn
+      if (k > 0) ok = mbar_wait_warp(q_free, (k - 1) & 1, abort_flag, DERR_WAIT_MMA);
+      if (!ok) break;
+#pragma unroll 1
+      for (int r = i; r < C::ROWS; r += C::CONV) {
+        const int row = it.row0 + r, tok = row / group;
+        const uint16_t* src = p.q + (it.t0 + tok) * p.ld_q + static_cast<size_t>(it.head * group + row % group) * D;
+        const bool live = row < it.rows;
+        float f = 1.f, down = 1.f;
+        if (p.c.bf16 && live) {
+          unsigned top = 0;
+          for (int d = 0; d < D; d += 8) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + d));
+            top = top2(top2(top2(top2(top, w.x), w.y), w.z), w.w);
+          }
+          const int e = exponent_down(max(top & 0xffffu, top >> 16), 1);
+          f = pow2f(e);
+          down = pow2f(-e);
+        }
+        for (int d = 0; d < D; d += 8) {
+          uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(src + d)) : make_uint4(0, 0, 0, 0);
+          if (p.c.bf16) w = scale8(w, 1, down);
+          *reinterpret_cast<uint4*>(smem + (r >> 7) * C::Q_BYTES + attn8_off<D>(128, r & 127, d)) = w;
+        }
+        reinterpret_cast<float*>(smem + C::OFF_QF)[(k & 1) * C::ROWS + r] = f * p.scale_log2;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+      uint32_t next_pages = tile_page(1);
+      for (int j = 0; j < it.nkt; ++j, ++g) {
+        const int st = g % C::ST, limit = it.full - 128 * j;
+        uint8_t* ks = smem + C::OFF_KV + st * 2 * C::KV_BYTES;
+        uint8_t* vs = ks + C::KV_BYTES;
+        float* key = reinterpret_cast<float*>(smem + C::OFF_KEY) + st * 3 * C::BN;
+        float ksc[2] = {0.f, 0.f}, vsc[2] = {0.f, 0.f};  // of keys i and i + 96
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int kt = min(i + C::CONV * n, 127);
+          const size_t ph = __shfl_sync(0xffffffffu, pages, kt >> psh);
+          if (kt < limit) {
+            ksc[n] = __ldg(p.c.k_scale + ph);
+            vsc[n] = __ldg(p.c.v_scale + ph);
+          }
+        }
+        if (g >= C::ST) ok = mbar_wait_warp(&kv_empty[st], (g / C::ST - 1) & 1, abort_flag, DERR_WAIT_MMA);
+        if (!ok) break;
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+          const int c = i + C::CONV * u, kt = c / NC, d = c % NC * 16;
+          if (c >= ALL) break;
+          if (kt < limit) {
+            uint4 a, b;
+            widen(kr[u].x, a.x, a.y);
+            widen(kr[u].y, a.z, a.w);
+            widen(kr[u].z, b.x, b.y);
+            widen(kr[u].w, b.z, b.w);
+            *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, kt, d)) = a;
+            *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, kt, d + 8)) = b;
+          }
+          const int vt = c / (D / 4) * 4, vd = c % (D / 4) * 4;
+          if (vt < limit) {
+            const __half2 off = __half2half2(__ushort_as_half(0x6480));
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {  // four channels of token vt + t
+              const uint32_t lo = __byte_perm(vr[u].x, vr[u].y, t | (4 + t) << 8);
+              const uint32_t hi = __byte_perm(vr[u].z, vr[u].w, t | (4 + t) << 8);
+              const uint32_t x = __byte_perm(lo, 0x64646464u, 0x4240), y = __byte_perm(hi, 0x64646464u, 0x4240);
+              const __half2 x2 = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
+              const __half2 y2 = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+              *reinterpret_cast<uint2*>(vs + attn8_off<D>(128, vt + t, vd)) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&x2), *reinterpret_cast<const uint32_t*>(&y2));
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int kt = i + C::CONV * n;
+          if (kt < min(limit, 128)) {
+            const float v = vsc[n] < 7.8886091e-31f ? 7.8886091e-31f : vsc[n];  // 2^-100 at least; NaN stays
+            key[kt] = ksc[n];
+            key[128 + kt] = log2f(v);
+            key[256 + kt] = v == v ? 1.f / v : 1.f;  // (NaN comes through the logarithm, to visible keys only)
+          }
+        }
+        if (limit < 128) {  // the newest block's tokens, and zeros past them
+          const int first = max(limit, 0), have = it.len - 128 * j;  // keys [first, have) of the tile
+          const int nrow = p.c.rows ? __ldg(p.c.rows + it.b) : it.b;
+          const bool good = nrow >= 0 && nrow < p.c.new_rows;
+          if (!good && i == 0) record_error(DERR_KV_RANGE);
+          const size_t base = ((static_cast<size_t>(good ? nrow : 0) * 2 + (it.full >> psh & 1)) * p.c.kv_heads + it.head) *
+                              static_cast<size_t>(P * D);
+          constexpr int LK = D / 8, TK = 32 / LK;  // lanes a token, tokens a warp
+          for (int t0 = first + cw * TK; t0 < 128; t0 += 3 * TK) {
+            const int t = t0 + lane / LK, d = lane % LK * 8;
+            const bool live = good && t < have;
+            uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(p.c.k_new + base + (t - first) * D + d)) : make_uint4(0, 0, 0, 0);
+            unsigned top = top2(top2(top2(top2(0u, w.x), w.y), w.z), w.w);
+            top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+            for (int x = 1; x < LK; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const int e = exponent_down(top, p.c.bf16);
+            if (t < 128) {
+              *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, t, d)) = scale8(w, p.c.bf16, pow2f(-e));
+              if (d == 0) key[t] = pow2f(e);
+            }
+          }
+          for (int t = first + 4 * cw; t < 128; t += 12) {  // four tokens a warp
+            constexpr int NV = D == 128 ? 2 : 1;             // 16-byte pieces (two channels of four tokens) a lane
+            uint4 w[NV];
+            unsigned top[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < NV; ++x) {
+              const int piece = lane + 32 * x;
+              w[x] = good && piece < D / 2 && t < have
+                         ? __ldg(reinterpret_cast<const uint4*>(p.c.v_new + base + (t - first) * D + piece * 8)) : make_uint4(0, 0, 0, 0);
+              const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const unsigned a = u[n >> 1] >> (16 * (n & 1)) & 0x7fffu, b = u[2 + (n >> 1)] >> (16 * (n & 1)) & 0x7fffu;
+                top[n] = max(top[n], max(a, b));
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              top[n] = __reduce_max_sync(0xffffffffu, top[n]);
+              const bool live = t + n < have, sane = h16_to_f(top[n], p.c.bf16) < INFINITY;
+              const int e = live ? exponent_down(top[n], p.c.bf16) : 0;
+              const float down = pow2f(-e);
+#pragma unroll
+              for (int x = 0; x < NV; ++x) {
+                const int piece = lane + 32 * x;
+                const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+                if (piece < D / 2) {
+                  const float a = h16_to_f(u[n >> 1] >> (16 * (n & 1)) & 0xffffu, p.c.bf16);
+                  const float b = h16_to_f(u[2 + (n >> 1)] >> (16 * (n & 1)) & 0xffffu, p.c.bf16);
+                  *reinterpret_cast<uint32_t*>(vs + attn8_off<D>(128, t + n, 2 * piece)) =
+                      live && sane ? pack_half2(a * down, b * down) : 0u;
+                }
+              }
+              if (lane == 0) {
+                key[128 + t + n] = sane ? static_cast<float>(e) : __uint_as_float(0x7fc00000u);
+                key[256 + t + n] = down;
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&kv_full[st]);
+        if (j + 1 < it.nkt) {
+          pages = next_pages;
+          fetch(j + 1, pages);
+          next_pages = tile_page(j + 2);
+        }
+      }
+      ++k;
+    }
+  } else {
+    const int x = (warp - 4) >> 2, rl = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + C::TM_O + x * D;
+    int g = 0, k = 0;
+    bool ok = true;
+    for (int at = blockIdx.x; ok && at < items; at += G) {
+      const Attn8Item it = attn8_item(p, line, at);
+      const int row = it.row0 + 128 * x + rl;
+      const int lim = attn8_limit(it, row, group), least = attn8_limit(it, it.row0 + 128 * x, group);
+      // rows past the sequence's see nothing, and mask every key
+      const bool ragged = it.row0 + 128 * x + 128 > it.rows;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < it.nkt; ++j) {
+        const int st = (g + j) % C::ST;
+        ok = mbar_wait_warp(&kv_full[st], (g + j) / C::ST & 1, abort_flag, DERR_WAIT_SLOT) &&
+             mbar_wait_warp(&s_full[x], (g + j) & 1, abort_flag, DERR_WAIT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        float s[128];
+        tmem_ld128(ts, s);
+        const float* key = reinterpret_cast<const float*>(smem + C::OFF_KEY) + st * 3 * C::BN;
+        const float qf = reinterpret_cast<const float*>(smem + C::OFF_QF)[(k & 1) * C::ROWS + 128 * x + rl];
+        const bool masked = ragged || 128 * j + 128 > least;
+        float alpha;
+        if (128 * j + 128 > it.full) attn8_weights<true>(s, key, qf, 128 * j, lim, masked, m, l, alpha);
+        else attn8_weights<false>(s, key, qf, 128 * j, lim, masked, m, l, alpha);
+        uint32_t pk[64];
+#pragma unroll
+        for (int c = 0; c < 64; ++c) pk[c] = pack_half2(s[2 * c], s[2 * c + 1]);
+        tmem_st64(ts, pk);
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            tmem_ld32(to + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= alpha;
+            tmem_st32(to + c, o);
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      if (it.nkt > 0) {
+        g += it.nkt;
+        ++k;
+        ok = mbar_wait_warp(&o_done[x], (g - 1) & 1, abort_flag, DERR_WAIT_MMA);
+        if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
+        tc_fence_after();
+      }
+      const float inv = lim > 0 ? 1.f / l : 0.f;  // a row that sees no key is 0
+      const int tok = row / group;
+      uint16_t* dst = p.out + (it.t0 + tok) * p.ld_out + static_cast<size_t>(it.head * group + row % group) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (it.nkt > 0) {
+          tmem_ld32(to + c, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (row < it.rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              w[n] = lim > 0 ? f_to_h16(o[e + 2 * n] * inv, p.c.bf16) | f_to_h16(o[e + 2 * n + 1] * inv, p.c.bf16) << 16 : 0u;
+            *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace b200

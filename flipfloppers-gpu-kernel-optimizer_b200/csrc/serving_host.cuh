@@ -2,7 +2,7 @@
 // the library's one translation unit (included by b200_block.cu, whose helpers it uses).
 #pragma once
 
-#include "attn8.cuh"
+#include "attn8_tile.cuh"
 #include "gemm_i8.cuh"
 
 namespace {
@@ -151,7 +151,26 @@ int launch_attn8(Attn8Params& p, long long rows, cudaStream_t st) {
 }
 
 template <int D>
+int launch_attn8_tile(Attn8Params& p, long long rows, cudaStream_t st) {
+  using C = Attn8TileCfg<D>;
+  auto kern = k_attn8_tile<D>;
+  constexpr int most = C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4 + 1024;
+  static_assert(most <= 227 * 1024, "tiles and line fit an SM");
+  if (int rc = set_smem(reinterpret_cast<const void*>(kern), most)) return rc;
+  const long long items = (rows / 256 + p.batch) * p.c.kv_heads;
+  launch_kernel(kern, dim3(static_cast<unsigned>(std::min<long long>(items, num_sms()))), dim3(C::THREADS),
+                C::TOTAL + (p.batch + 1) * 4 + 1024, st, p);
+  return launch_status();
+}
+
+// Whether the 256-row tcgen05 kernel is ahead of the warps' streams: rows (new tokens times the group) in all.
+bool attn8_many_rows(long long rows, int kv_heads, int batch, int head_dim) {
+  return rows / batch >= 128 && rows * kv_heads * head_dim >= 300000;
+}
+
+template <int D>
 int launch_attn8_d(Attn8Params& p, bool one, long long rows, cudaStream_t st) {
+  if (attn8_many_rows(rows, p.c.kv_heads, p.batch, D)) return launch_attn8_tile<D>(p, rows, st);
   if (p.c.page == 16) return one ? launch_attn8<D, 1, true>(p, rows, st) : launch_attn8<D, 2, true>(p, rows, st);
   return one ? launch_attn8<D, 1, false>(p, rows, st) : launch_attn8<D, 2, false>(p, rows, st);
 }

@@ -313,6 +313,70 @@ def test_attend_many_chunks_of_rows(sv):
     m.check_attend(q, [2500, 1500, 1300, 1], 16)
 
 
+PROMPTS = [  # page, dim, kv, group, lens before, new tokens: enough rows for the 256-row kernel
+    (64, 64, 8, 1, [0, 129], [640, 257]),
+    (128, 128, 4, 2, [1000, 0], [300, 511]),
+    (16, 32, 8, 3, [7, 300], [401, 255]),
+    (32, 128, 2, 5, [63], [301]),
+    (16, 64, 16, 1, [0, 0, 33], [1, 385, 700]),
+    (128, 32, 8, 8, [4000], [200]),
+    (32, 64, 4, 4, [31, 500], [333, 0]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(PROMPTS)))
+def test_attend_prompts(sv, pkg, case, dtype):
+    page, dim, kv, group, before, new = PROMPTS[case]
+    assert sum(new) * group // len(new) >= 128 and sum(new) * group * kv * dim >= 300000  # the launcher's rule
+    m = Model(sv, len(before), kv, dim, page, max(a + b for a, b in zip(before, new)), dtype, seed=50 + case)
+    if sum(before):
+        m.append(before, kv * group)
+    q = m.append(new, kv * group)
+    a = m.check_attend(q, new, kv * group)
+    assert torch.equal(a, m.check_attend(q, new, kv * group))
+    assert pkg.runtime.device_error() == 0
+
+
+def test_prompt_rows_without_keys(sv):
+    """More new rows than cached tokens: the first rows see nothing."""
+    m = Model(sv, 2, 8, 64, 16, 512, torch.float16)
+    m.append([300, 0], 8)
+    q = m.rows(1200, 8 * 64).view(1200, 8, 64)
+    out = m.check_attend(q, [600, 600], 8)
+    assert not bool(out[:300].any()) and not bool(out[600:].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_prompt_scales_far_apart(sv, dtype):
+    """Blocks of very different sizes and of zeros, rows of any size, in the 256-row kernel."""
+    m = Model(sv, 1, 8, 64, 32, 1024, dtype)
+    x = m.rows(1000, 24 * 64)
+    x[:, 1024:] *= (torch.arange(1000, device="cuda") // 32 % 5).to(dtype)[:, None] * 0.25
+    x[128:256, 512:] *= 2 ** -6
+    x[256:288, 512:] = 0
+    x[:32, 1024:] = 0
+    x[990:, 1024:] *= 2 ** -5
+    q = m.append([1000], 8, qkv=x)
+    m.check_attend(q, [1000], 8)
+
+
+def test_prompt_nan_stays_with_the_rows_that_see_it(sv):
+    m = Model(sv, 1, 8, 64, 64, 1024, torch.float16)
+    x = m.rows(1000, 24 * 64)
+    clean = x.clone()
+    x[400, 1024 + 7] = float("nan")  # a value of head 0: block 6 is NaN as a whole
+    x[990, 1024 + 70] = float("inf")  # a value of head 1 in the newest block
+    x[980, 512 + 128] = float("nan")  # a key of head 2 in the newest block
+    out = m.c.attend(m.c.append(x, starts([1000]), i32([0]), heads=8), starts([1000]), i32([1000]), max_q_len=1000)
+    q = m.append([1000], 8, qkv=clean, start=[0])
+    want = m.check_attend(q, [1000], 8)
+    assert torch.equal(out[:384, 0], want[:384, 0]) and bool(out[384:, 0].isnan().all())
+    assert torch.equal(out[:990, 1], want[:990, 1]) and not bool(out[990:, 1].isfinite().any())
+    assert torch.equal(out[:980, 2], want[:980, 2]) and bool(out[980:, 2].isnan().all())
+    assert torch.equal(out[:, 3:], want[:, 3:])
+
+
 def test_rows_without_keys_are_zero(sv):
     """Queries of tokens before the sequence's first key (lens < new tokens), and an empty sequence."""
     m = Model(sv, 3, 1, 64, 16, 64, torch.float16)
