@@ -18,6 +18,8 @@
 // Bound: the exponentials (16 a clock and SM), 2048 clocks for two 128x128 tiles.
 #pragma once
 
+#include <type_traits>
+
 #include "attn8.cuh"
 
 namespace b200 {
@@ -91,66 +93,70 @@ __device__ __forceinline__ uint4 scale8(uint4 w, int bf16, float f) {  // eight 
 }
 __device__ __forceinline__ unsigned top2(unsigned top, uint32_t w) { return __vmaxu2(top, w & 0x7fff7fffu); }
 
-// One softmax step of a row: raw scores s (in registers), key factors in shared memory.
-template <bool EACH>  // EACH: factors differ key by key (the newest block's tile), else every 16 keys
-__device__ __forceinline__ void attn8_weights(float (&s)[128], const float* key, float qf, int k0, int lim, bool masked, float& m,
-                                              float& l, float& alpha) {
+// One softmax step of a row: raw scores s (in registers) become weights.  Key factors in shared memory: K scale,
+// log2 of the V scale, 1 / V scale.
+// A tile of full blocks that the row sees whole: the factors are alike for 16 keys, and with f > 0 a group's
+// maximum is that of its raw scores, so that one multiply-add a score is all there is beside the exponential.
+__device__ __forceinline__ void attn8_weights(float (&s)[128], const float* key, float qf, float& m, float& l, float& alpha) {
+  float f[8], v[8], now = m;
 #pragma unroll
   for (int g = 0; g < 8; ++g) {
-    if constexpr (EACH) {
-#pragma unroll
-      for (int c = 16 * g; c < 16 * g + 16; c += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(key + c), v = *reinterpret_cast<const float4*>(key + 128 + c);
-        s[c] = fmaf(s[c], f.x * qf, v.x);
-        s[c + 1] = fmaf(s[c + 1], f.y * qf, v.y);
-        s[c + 2] = fmaf(s[c + 2], f.z * qf, v.z);
-        s[c + 3] = fmaf(s[c + 3], f.w * qf, v.w);
-      }
-    } else {
-      const float f = key[16 * g] * qf, v = key[128 + 16 * g];
-      const uint64_t f2 = f2pk(f, f), v2 = f2pk(v, v);
-#pragma unroll
-      for (int c = 16 * g; c < 16 * g + 16; c += 2) f2upk(f2fma(f2pk(s[c], s[c + 1]), f2, v2), s[c], s[c + 1]);
-    }
+    f[g] = key[16 * g] * qf;
+    v[g] = key[128 + 16 * g];
+    float x = fmax3(s[16 * g], s[16 * g + 1], s[16 * g + 2]), y = fmax3(s[16 * g + 3], s[16 * g + 4], s[16 * g + 5]);
+    x = fmax3(x, s[16 * g + 6], s[16 * g + 7]);
+    y = fmax3(y, s[16 * g + 8], s[16 * g + 9]);
+    x = fmax3(x, s[16 * g + 10], s[16 * g + 11]);
+    y = fmax3(y, s[16 * g + 12], s[16 * g + 13]);
+    now = fmaxf(now, fmaf(fmaxf(fmax3(x, s[16 * g + 14], s[16 * g + 15]), y), f[g], v[g]));
   }
-  if (masked) {
+  const float most = now == -INFINITY ? 0.f : now, ref = most - ATTN8_LIFT;
+  alpha = fast_exp2(m - most);
+  m = now;
+  float sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < 128; ++c)
-      if (k0 + c >= lim) s[c] = -INFINITY;
+  for (int g = 0; g < 8; ++g) {
+    const uint64_t f2 = f2pk(f[g], f[g]), v2 = f2pk(v[g] - ref, v[g] - ref);
+    uint64_t a0 = f2pk(0.f, 0.f), a1 = a0;
+#pragma unroll
+    for (int c = 16 * g; c < 16 * g + 16; c += 4) {
+      float x, y, z, w;
+      f2upk(f2fma(f2pk(s[c], s[c + 1]), f2, v2), x, y);
+      f2upk(f2fma(f2pk(s[c + 2], s[c + 3]), f2, v2), z, w);
+      s[c] = fast_exp2(x); s[c + 1] = fast_exp2(y); s[c + 2] = fast_exp2(z); s[c + 3] = fast_exp2(w);
+      a0 = f2add(a0, f2pk(s[c], s[c + 1]));
+      a1 = f2add(a1, f2pk(s[c + 2], s[c + 3]));
+    }
+    float x, y;
+    f2upk(f2add(a0, a1), x, y);
+    sum = fmaf(x + y, key[256 + 16 * g], sum);
+  }
+  l = l * alpha + sum;
+}
+// The general form: factors key by key, keys from lim on hidden.
+__device__ __forceinline__ void attn8_weights_each(float (&s)[128], const float* key, float qf, int k0, int lim, float& m, float& l,
+                                                   float& alpha) {
+#pragma unroll
+  for (int c = 0; c < 128; c += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(key + c), v = *reinterpret_cast<const float4*>(key + 128 + c);
+    s[c] = k0 + c < lim ? fmaf(s[c], f.x * qf, v.x) : -INFINITY;
+    s[c + 1] = k0 + c + 1 < lim ? fmaf(s[c + 1], f.y * qf, v.y) : -INFINITY;
+    s[c + 2] = k0 + c + 2 < lim ? fmaf(s[c + 2], f.z * qf, v.z) : -INFINITY;
+    s[c + 3] = k0 + c + 3 < lim ? fmaf(s[c + 3], f.w * qf, v.w) : -INFINITY;
   }
   const float now = fmaxf(m, row_max<128>(s));
   const float most = now == -INFINITY ? 0.f : now, ref = most - ATTN8_LIFT;
   alpha = fast_exp2(m - most);
   m = now;
-  const uint64_t nr = f2pk(-ref, -ref);
   float sum = 0.f;
 #pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    if constexpr (EACH) {
-#pragma unroll
-      for (int c = 16 * g; c < 16 * g + 16; c += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(key + 256 + c);
-        s[c] = fast_exp2(s[c] - ref);
-        s[c + 1] = fast_exp2(s[c + 1] - ref);
-        s[c + 2] = fast_exp2(s[c + 2] - ref);
-        s[c + 3] = fast_exp2(s[c + 3] - ref);
-        sum = fmaf(s[c], v.x, fmaf(s[c + 1], v.y, fmaf(s[c + 2], v.z, fmaf(s[c + 3], v.w, sum))));
-      }
-    } else {
-      uint64_t a0 = f2pk(0.f, 0.f), a1 = a0;
-#pragma unroll
-      for (int c = 16 * g; c < 16 * g + 16; c += 4) {
-        float x, y, z, w;
-        f2upk(f2add(f2pk(s[c], s[c + 1]), nr), x, y);
-        f2upk(f2add(f2pk(s[c + 2], s[c + 3]), nr), z, w);
-        s[c] = fast_exp2(x); s[c + 1] = fast_exp2(y); s[c + 2] = fast_exp2(z); s[c + 3] = fast_exp2(w);
-        a0 = f2add(a0, f2pk(s[c], s[c + 1]));
-        a1 = f2add(a1, f2pk(s[c + 2], s[c + 3]));
-      }
-      float x, y;
-      f2upk(f2add(a0, a1), x, y);
-      sum = fmaf(x + y, key[256 + 16 * g], sum);
-    }
+  for (int c = 0; c < 128; c += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(key + 256 + c);
+    s[c] = fast_exp2(s[c] - ref);
+    s[c + 1] = fast_exp2(s[c + 1] - ref);
+    s[c + 2] = fast_exp2(s[c + 2] - ref);
+    s[c + 3] = fast_exp2(s[c + 3] - ref);
+    sum = fmaf(s[c], v.x, fmaf(s[c + 1], v.y, fmaf(s[c + 2], v.z, fmaf(s[c + 3], v.w, sum))));
   }
   l = l * alpha + sum;
 }
@@ -254,33 +260,29 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         const int nkt = attn8_item(p, line, at).nkt;
         if (nkt == 0) continue;
         if (!mbar_wait(q_full, k & 1, abort_flag, DERR_WAIT_SLOT)) break;
-        for (int j = 0; ok && j <= nkt; ++j) {
-          // PV of tile j - 1 and S of tile j, for each row tile; S overwrites the P that the PV has read
-          if (j < nkt) {
-            ok = mbar_wait(&kv_full[(g + j) % C::ST], (g + j) / C::ST & 1, abort_flag, DERR_WAIT_SLOT);
-            if (!ok) break;
-          }
+        // S overwrites the P that the PV before it has read: it waits for that PV.
+        auto scores = [&](int x, int n) {  // of key tile n (counted over items)
+          if (n > 0 && !mbar_wait(&o_done[x], (n - 1) & 1, abort_flag, DERR_WAIT_MMA)) return false;
+          tc_fence_after();
+          issue_s(x, n % C::ST);
+          return true;
+        };
+        ok = mbar_wait(&kv_full[g % C::ST], g / C::ST & 1, abort_flag, DERR_WAIT_SLOT) && scores(0, g) && scores(1, g);
+        if (ok && nkt == 1) tc_commit(q_free);
+        for (int j = 0; ok && j < nkt; ++j) {
+          const int n = g + j;
+          const bool more = j + 1 < nkt;
           for (int x = 0; ok && x < 2; ++x) {
-            if (j > 0) {
-              ok = mbar_wait(&p_full[x], (g + j - 1) & 1, abort_flag, DERR_WAIT_SOFTMAX);
-              if (!ok) break;
-              tc_fence_after();
-              issue_pv(x, (g + j - 1) % C::ST, j == 1);
-              if (x == 1) tc_commit(&kv_empty[(g + j - 1) % C::ST]);
-              if (j < nkt) {
-                ok = mbar_wait(&o_done[x], (g + j - 1) & 1, abort_flag, DERR_WAIT_MMA);
-                if (!ok) break;
-              }
-            } else if (g > 0) {
-              ok = mbar_wait(&o_done[x], (g - 1) & 1, abort_flag, DERR_WAIT_MMA);
-              if (!ok) break;
-            }
-            if (j < nkt) {
-              tc_fence_after();
-              issue_s(x, (g + j) % C::ST);
-              if (x == 1 && j == nkt - 1) tc_commit(q_free);
-            }
+            ok = mbar_wait(&p_full[x], n & 1, abort_flag, DERR_WAIT_SOFTMAX);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(x, n % C::ST, j == 0);
+            if (x == 1) tc_commit(&kv_empty[n % C::ST]);
+            if (more)
+              ok = (x == 1 || mbar_wait(&kv_full[(n + 1) % C::ST], (n + 1) / C::ST & 1, abort_flag, DERR_WAIT_SLOT)) &&
+                   scores(x, n + 1);
           }
+          if (ok && j + 2 == nkt) tc_commit(q_free);
         }
         g += nkt;
         ++k;
@@ -300,33 +302,47 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
     for (int at = blockIdx.x; ok && at < items; at += G) {
       const Attn8Item it = attn8_item(p, line, at);
       if (it.nkt == 0) continue;
-      // page of block `blk` of the sequence (those in full blocks)
-      auto page_of = [&](int blk) -> size_t {
-        int id = __ldg(p.c.table + static_cast<size_t>(it.b) * p.c.table_width + blk);
+      // a tile's pages, one a lane: the table's entries a tile ahead of the codes, checked when they are used
+      auto tile_entry = [&](int j) {
+        const int blk = (j << (7 - psh)) + lane;
+        return lane < (128 >> psh) && blk < (it.full >> psh)
+                   ? __ldg(p.c.table + static_cast<size_t>(it.b) * p.c.table_width + blk) : 0;
+      };
+      auto tile_page = [&](int id) {
         if (id < 0 || id >= p.c.num_pages) {
           record_error(DERR_KV_RANGE);
           id = 0;
         }
-        return static_cast<size_t>(id) * p.c.kv_heads + it.head;
+        return static_cast<uint32_t>(id) * p.c.kv_heads + it.head;
       };
-      // a tile's pages, one a lane, a tile ahead of its codes
-      auto tile_page = [&](int j) {
-        const int blk = (j << (7 - psh)) + lane;
-        return lane < (128 >> psh) && blk < (it.full >> psh) ? static_cast<uint32_t>(page_of(blk)) : 0u;
+      // byte offset of a key's first code in the pools
+      auto block = [&](uint32_t pages, int key) {
+        return static_cast<uint64_t>(__shfl_sync(0xffffffffu, pages, key >> psh)) * static_cast<uint32_t>(P * D) +
+               static_cast<uint32_t>((key & (P - 1)) * D);
       };
-      auto fetch = [&](int j, uint32_t pages) {
-        const int limit = it.full - 128 * j;  // keys of the tile in full blocks
+      auto fetch = [&](uint32_t pages) {
 #pragma unroll
-        for (int u = 0; u < MINE; ++u) {
+        for (int u = 0; u < MINE; ++u) {  // (past the full blocks: some page's codes, which are not used)
           const int c = min(i + C::CONV * u, ALL - 1), kt = c / NC, vt = c / (D / 4) * 4;
-          const size_t ka = static_cast<size_t>(__shfl_sync(0xffffffffu, pages, kt >> psh)) * P * D + (kt & (P - 1)) * D + c % NC * 16;
-          const size_t va = static_cast<size_t>(__shfl_sync(0xffffffffu, pages, vt >> psh)) * P * D + (vt & (P - 1)) * D + c % (D / 4) * 16;
-          kr[u] = kt < limit ? __ldg(reinterpret_cast<const uint4*>(p.c.k_pages + ka)) : make_uint4(0, 0, 0, 0);
-          vr[u] = vt < limit ? __ldg(reinterpret_cast<const uint4*>(p.c.v_pages + va)) : make_uint4(0, 0, 0, 0);
+          const size_t ka = block(pages, kt) + c % NC * 16;
+          const size_t va = block(pages, vt) + c % (D / 4) * 16;
+          kr[u] = __ldg(reinterpret_cast<const uint4*>(p.c.k_pages + ka));
+          vr[u] = __ldg(reinterpret_cast<const uint4*>(p.c.v_pages + va));
         }
       };
-      uint32_t pages = tile_page(0);
-      fetch(0, pages);
+      // codes of a tile into L2, two tiles ahead of their use
+      auto prefetch = [&](int j, uint32_t pages) {
+        for (int c = i; c < D; c += C::CONV) {  // 128 bytes of K and of V each
+          const int kt = c * 128 / D;           // the key they begin with
+          const size_t at = block(pages, kt) + c * 128 % D;
+          if (kt < it.full - 128 * j) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.c.k_pages + at));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.c.v_pages + at));
+          }
+        }
+      };
+      uint32_t pages = tile_page(tile_entry(0)), pages1 = tile_page(tile_entry(1));
+      fetch(pages);
       // Q: rows in turn
       if (k > 0) ok = mbar_wait_warp(q_free, (k - 1) & 1, abort_flag, DERR_WAIT_MMA);
       if (!ok) break;
@@ -355,52 +371,57 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
       }
       fence_proxy_async_smem();
       mbar_arrive(q_full);
-      uint32_t next_pages = tile_page(1);
+      prefetch(1, pages1);
+      int next = tile_entry(2);
       for (int j = 0; j < it.nkt; ++j, ++g) {
         const int st = g % C::ST, limit = it.full - 128 * j;
         uint8_t* ks = smem + C::OFF_KV + st * 2 * C::KV_BYTES;
         uint8_t* vs = ks + C::KV_BYTES;
         float* key = reinterpret_cast<float*>(smem + C::OFF_KEY) + st * 3 * C::BN;
-        float ksc[2] = {0.f, 0.f}, vsc[2] = {0.f, 0.f};  // of keys i and i + 96
+        float ksc[2], vsc[2];  // of keys i and i + 96
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int kt = min(i + C::CONV * n, 127);
           const size_t ph = __shfl_sync(0xffffffffu, pages, kt >> psh);
-          if (kt < limit) {
-            ksc[n] = __ldg(p.c.k_scale + ph);
-            vsc[n] = __ldg(p.c.v_scale + ph);
-          }
+          ksc[n] = __ldg(p.c.k_scale + ph);
+          vsc[n] = __ldg(p.c.v_scale + ph);
         }
         if (g >= C::ST) ok = mbar_wait_warp(&kv_empty[st], (g / C::ST - 1) & 1, abort_flag, DERR_WAIT_MMA);
         if (!ok) break;
+        // the codes as whole numbers; whole tiles without a branch for every chunk
+        auto widen_tile = [&](auto every) {
+          constexpr bool whole = decltype(every)::value;
 #pragma unroll
-        for (int u = 0; u < MINE; ++u) {
-          const int c = i + C::CONV * u, kt = c / NC, d = c % NC * 16;
-          if (c >= ALL) break;
-          if (kt < limit) {
-            uint4 a, b;
-            widen(kr[u].x, a.x, a.y);
-            widen(kr[u].y, a.z, a.w);
-            widen(kr[u].z, b.x, b.y);
-            widen(kr[u].w, b.z, b.w);
-            *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, kt, d)) = a;
-            *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, kt, d + 8)) = b;
-          }
-          const int vt = c / (D / 4) * 4, vd = c % (D / 4) * 4;
-          if (vt < limit) {
-            const __half2 off = __half2half2(__ushort_as_half(0x6480));
+          for (int u = 0; u < MINE; ++u) {
+            const int c = i + C::CONV * u, kt = c / NC, d = c % NC * 16;
+            if (MINE * C::CONV > ALL && u == MINE - 1 && c >= ALL) break;
+            if (whole || kt < limit) {
+              uint4 a, b;
+              widen(kr[u].x, a.x, a.y);
+              widen(kr[u].y, a.z, a.w);
+              widen(kr[u].z, b.x, b.y);
+              widen(kr[u].w, b.z, b.w);
+              *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, kt, d)) = a;
+              *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, kt, d + 8)) = b;
+            }
+            const int vt = c / (D / 4) * 4, vd = c % (D / 4) * 4;
+            if (whole || vt < limit) {
+              const __half2 off = __half2half2(__ushort_as_half(0x6480));
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {  // four channels of token vt + t
-              const uint32_t lo = __byte_perm(vr[u].x, vr[u].y, t | (4 + t) << 8);
-              const uint32_t hi = __byte_perm(vr[u].z, vr[u].w, t | (4 + t) << 8);
-              const uint32_t x = __byte_perm(lo, 0x64646464u, 0x4240), y = __byte_perm(hi, 0x64646464u, 0x4240);
-              const __half2 x2 = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
-              const __half2 y2 = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
-              *reinterpret_cast<uint2*>(vs + attn8_off<D>(128, vt + t, vd)) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&x2), *reinterpret_cast<const uint32_t*>(&y2));
+              for (int t = 0; t < 4; ++t) {  // four channels of token vt + t
+                const uint32_t lo = __byte_perm(vr[u].x, vr[u].y, t | (4 + t) << 8);
+                const uint32_t hi = __byte_perm(vr[u].z, vr[u].w, t | (4 + t) << 8);
+                const uint32_t x = __byte_perm(lo, 0x64646464u, 0x4240), y = __byte_perm(hi, 0x64646464u, 0x4240);
+                const __half2 x2 = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
+                const __half2 y2 = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+                *reinterpret_cast<uint2*>(vs + attn8_off<D>(128, vt + t, vd)) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&x2), *reinterpret_cast<const uint32_t*>(&y2));
+              }
             }
           }
-        }
+        };
+        if (limit >= 128) widen_tile(std::true_type{});
+        else widen_tile(std::false_type{});
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int kt = i + C::CONV * n;
@@ -476,9 +497,11 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         fence_proxy_async_smem();
         mbar_arrive(&kv_full[st]);
         if (j + 1 < it.nkt) {
-          pages = next_pages;
-          fetch(j + 1, pages);
-          next_pages = tile_page(j + 2);
+          pages = pages1;
+          pages1 = tile_page(next);  // (before the codes are asked for: a wait for it could be a wait for them)
+          next = tile_entry(j + 3);
+          prefetch(j + 2, pages1);
+          fetch(pages);
         }
       }
       ++k;
@@ -493,8 +516,8 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
       const Attn8Item it = attn8_item(p, line, at);
       const int row = it.row0 + 128 * x + rl;
       const int lim = attn8_limit(it, row, group), least = attn8_limit(it, it.row0 + 128 * x, group);
-      // rows past the sequence's see nothing, and mask every key
-      const bool ragged = it.row0 + 128 * x + 128 > it.rows;
+      // rows past the sequence's see nothing, and hide every key (a factor that is not positive needs the general form)
+      const bool ragged = it.row0 + 128 * x + 128 > it.rows || !(p.scale_log2 > 0.f);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < it.nkt; ++j) {
         const int st = (g + j) % C::ST;
@@ -506,10 +529,9 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         tmem_ld128(ts, s);
         const float* key = reinterpret_cast<const float*>(smem + C::OFF_KEY) + st * 3 * C::BN;
         const float qf = reinterpret_cast<const float*>(smem + C::OFF_QF)[(k & 1) * C::ROWS + 128 * x + rl];
-        const bool masked = ragged || 128 * j + 128 > least;
         float alpha;
-        if (128 * j + 128 > it.full) attn8_weights<true>(s, key, qf, 128 * j, lim, masked, m, l, alpha);
-        else attn8_weights<false>(s, key, qf, 128 * j, lim, masked, m, l, alpha);
+        if (ragged || 128 * j + 128 > min(least, it.full)) attn8_weights_each(s, key, qf, 128 * j, lim, m, l, alpha);
+        else attn8_weights(s, key, qf, m, l, alpha);
         uint32_t pk[64];
 #pragma unroll
         for (int c = 0; c < 64; ++c) pk[c] = pack_half2(s[2 * c], s[2 * c + 1]);
