@@ -106,6 +106,7 @@ struct GemmI8Params {
   long long ld_resid;
   void* out;           // [M, N], row stride ld_out
   long long ld_out;
+  int vec_resid;       // resid's rows are 16-byte aligned
   int tma_out;         // out's rows are 16-byte aligned: tiles leave by TMA store
 };
 
@@ -164,8 +165,16 @@ __device__ __forceinline__ void i8_epilogue(const CUtensorMap* tmO, const GemmI8
       if (row < p.M) {
         const float* r = p.resid + row * p.ld_resid + col;
         float u[CC];
+        if (p.vec_resid && col + CC <= p.N) {
 #pragma unroll
-        for (int j = 0; j < CC; ++j) u[j] = col + j < p.N ? __ldg(r + j) : 0.f;
+          for (int j = 0; j < CC; j += 4) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(r + j));
+            u[j] = w.x; u[j + 1] = w.y; u[j + 2] = w.z; u[j + 3] = w.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < CC; ++j) u[j] = col + j < p.N ? __ldg(r + j) : 0.f;
+        }
 #pragma unroll
         for (int j = 0; j < CC; ++j)
           v[j] = __fadd_rn(u[j], __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(__float_as_int(v[j])), sx), cols[c + j]),
@@ -359,11 +368,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 
 // The same on CTA pairs, after k_gemm2_tn: one 256x256 tile a pair, each CTA staging its 128 rows of x's codes and
 // 128 rows of w per 128-byte K slice.
-constexpr int GEMM2_I8_STAGES = 5;
-constexpr int GEMM2_I8_EW = 8;
+__host__ __device__ constexpr int gemm2_i8_stages(int ew) { return ew == 16 ? 4 : 5; }
+template <int EW>
 struct Gemm2I8Smem {
   static constexpr int A_BYTES = 128 * 128, STAGE_BYTES = 2 * A_BYTES;
-  static constexpr int STG_OFF = GEMM2_I8_STAGES * STAGE_BYTES, BAR_OFF = STG_OFF + GEMM2_I8_EW * I8_STG_WARP;
+  static constexpr int STG_OFF = gemm2_i8_stages(EW) * STAGE_BYTES, BAR_OFF = STG_OFF + EW * I8_STG_WARP;
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
 };
 __device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -376,12 +385,12 @@ __device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t adesc,
         "r"(0u), "r"(0u), "r"(0u), "r"(0u)
       : "memory");
 }
-template <int DT, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * GEMM2_I8_EW, 1)
+template <int DT, int EPI, int EW>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
     k_gemm2_i8(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                const __grid_constant__ CUtensorMap tmO, const GemmI8Params p) {
-  constexpr int STAGES = GEMM2_I8_STAGES, EW = GEMM2_I8_EW;
-  using L = Gemm2I8Smem;
+  constexpr int STAGES = gemm2_i8_stages(EW), CW = 256 / (EW / 4);  // columns a warp
+  using L = Gemm2I8Smem<EW>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align1024(smem_raw);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
@@ -488,12 +497,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * GEMM2_I8_E
     for (int i = 0; i < my_tiles; ++i) {
       const int b = i & 1;
       const int t = cid + i * ncl;
-      const int row0 = (t / ntl) * 256 + 128 * static_cast<int>(rank) + q * 32, col0 = (t % ntl) * 256 + part * 128;
+      const int row0 = (t / ntl) * 256 + 128 * static_cast<int>(rank) + q * 32, col0 = (t % ntl) * 256 + part * CW;
       i8_columns(p, col0, reinterpret_cast<float*>(stg + 4096), lane);
       const bool ok = mbar_wait_warp(&acc_full[b], (i >> 1) & 1, abort_flag, DERR_WAIT_MMA);
       if (!ok || *abort_flag) break;
       tc_fence_after();
-      i8_epilogue<DT, EPI>(&tmO, p, tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + part * 128, 128, col0, row0,
+      i8_epilogue<DT, EPI>(&tmO, p, tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + part * CW, CW, col0, row0,
                            stg, gc, lane);
       tc_fence_before();
       __syncwarp();

@@ -261,13 +261,20 @@ int launch_gemm_i8(const GemmI8Params& p, const CUtensorMap& ta, const void* w, 
       return rc;
   if (int rc = make_map_i8(&tw, w, p.N, p.K, ld_w, 128)) return rc;
   if (p.M >= 512 && p.N >= 256) {
-    auto kern = k_gemm2_i8<DT, EPI>;
-    if (int rc = set_smem(reinterpret_cast<const void*>(kern), Gemm2I8Smem::TOTAL)) return rc;
     const long long tiles = static_cast<long long>((p.M + 255) / 256) * ((p.N + 255) / 256);
     if (tiles > 0x3fffffffLL) return B200_ERR_TILE;
-    launch_kernel(kern, dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, num_sms() / 2))),
-                  dim3(64 + 32 * GEMM2_I8_EW), Gemm2I8Smem::TOTAL, st, ta, tw, to, p);
-    return launch_status();
+    const dim3 grid(2 * static_cast<unsigned>(std::min<long long>(tiles, num_sms() / 2)));
+    auto run = [&](auto kern, int ew, int smem) {
+      if (int rc = set_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
+      launch_kernel(kern, grid, dim3(64 + 32 * ew), smem, st, ta, tw, to, p);
+      return launch_status();
+    };
+    // 16 epilogue warps where the epilogue sets the speed, GELU over a short K (quantizer included: 32768x1024x4096
+    // 171 us, with 8 warps 178; 65536x256x1024 86 against 94), 8 and a deeper ring elsewhere (16384x2048x2048 GELU
+    // 80 against 82; 32768x1024x4096 without GELU 145 against 149)
+    if constexpr (EPI == I8_GELU)
+      if (p.K <= 1024) return run(k_gemm2_i8<DT, EPI, 16>, 16, Gemm2I8Smem<16>::TOTAL);
+    return run(k_gemm2_i8<DT, EPI, 8>, 8, Gemm2I8Smem<8>::TOTAL);
   }
   constexpr int BN = 128, STAGES = 5;
   using L = GemmI8Smem<BN, STAGES>;
@@ -335,6 +342,7 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   p.bias = a->bias;
   p.resid = a->resid;
   p.ld_resid = a->ld_resid;
+  p.vec_resid = a->resid && al16(a->resid) && a->ld_resid % 4 == 0;
   p.out = a->out;
   p.ld_out = a->ld_out;
   if (few) return launch_lin_small(p, a, st);
