@@ -23,7 +23,10 @@ library's equivalents:
   ``[B, S, H*hd]`` fp16 tensors (prefix-causal when ``q_offset > 0``: query i
   sits at key position ``q_offset + i``);
 * ``b200::block_megakernel(x, <stacked layer weights>, ...)`` -- the whole
-  small-model forward in one kernel (``k_block_small``).
+  small-model forward in one kernel (``k_block_small``);
+* ``b200::linear_int8`` -- ``serving.linear_int8``: rows quantized to 8 bits times an int8 weight;
+* ``b200::kv8_append`` / ``kv8_read`` / ``kv8_attention`` -- ``serving.PagedKV8``'s calls on the
+  cache's tensors (append writes the six cache tensors in place).
 
 Every op runs the library's kernels; CPU tensors are rejected (the ops are
 registered for CUDA only), there is no fallback.
@@ -37,6 +40,7 @@ import torch
 from torch import Tensor
 
 from . import runtime as rt
+from . import serving
 
 EPI_BIAS_F16 = rt.EPI_BIAS_F16
 EPI_BIAS_GELU_F16 = rt.EPI_BIAS_GELU_F16
@@ -202,3 +206,61 @@ def block_megakernel(x: Tensor, ln1_w: Tensor, ln1_b: Tensor, w_qkv: Tensor, b_q
 def _block_megakernel_fake(x, ln1_w, ln1_b, w_qkv, b_qkv, w_o, b_o, ln2_w, ln2_b, w_in, b_in, w_out, b_out, lnf_w,
                            lnf_b, num_heads, eps, causal, row_valid):
     return torch.empty_like(x)
+
+
+# ------------------------------------------------------------------ 8-bit serving
+@torch.library.custom_op("b200::linear_int8", mutates_args=(), device_types="cuda")
+def linear_int8(x: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor], gelu: bool, resid: Optional[Tensor],
+                out_f32: bool) -> Tensor:
+    """serving.linear_int8; the result is fp32 with ``resid`` or ``out_f32``, else of x's type."""
+    return serving.linear_int8(x, w, w_scale, bias, gelu=gelu, resid=resid, out_dtype=torch.float32 if out_f32 else None)
+
+
+@linear_int8.register_fake
+def _linear_int8_fake(x, w, w_scale, bias, gelu, resid, out_f32):
+    return x.new_empty((x.shape[0], w.shape[0]), dtype=torch.float32 if out_f32 or resid is not None else x.dtype)
+
+
+@torch.library.custom_op("b200::kv8_append", device_types="cuda",
+                         mutates_args=("k_pages", "v_pages", "k_scale", "v_scale", "k_newest", "v_newest"))
+def kv8_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale: Tensor, v_scale: Tensor, k_newest: Tensor,
+               v_newest: Tensor, table: Tensor, rows: Optional[Tensor], cu: Tensor, start: Tensor, heads: int,
+               cos: Optional[Tensor], sin: Optional[Tensor], interleaved: bool) -> Tensor:
+    """serving.PagedKV8.append on the cache's tensors; returns the rotated queries."""
+    cache = serving.PagedKV8(k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows)
+    return cache.append(qkv, cu, start, heads=heads, cos=cos, sin=sin, interleaved=interleaved)
+
+
+@kv8_append.register_fake
+def _kv8_append_fake(qkv, k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows, cu, start, heads, cos, sin,
+                     interleaved):
+    return qkv.new_empty((qkv.shape[0], heads, k_pages.shape[3]))
+
+
+@torch.library.custom_op("b200::kv8_read", mutates_args=(), device_types="cuda")
+def kv8_read(k_pages: Tensor, v_pages: Tensor, k_scale: Tensor, v_scale: Tensor, k_newest: Tensor, v_newest: Tensor,
+             table: Tensor, rows: Optional[Tensor], cu: Tensor, start: Tensor, lens: Tensor,
+             total: int) -> tuple[Tensor, Tensor]:
+    """serving.PagedKV8.read on the cache's tensors."""
+    cache = serving.PagedKV8(k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows)
+    return cache.read(cu, start, lens, total=total)
+
+
+@kv8_read.register_fake
+def _kv8_read_fake(k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows, cu, start, lens, total):
+    shape = (total, k_pages.shape[1], k_pages.shape[3])
+    return k_newest.new_empty(shape), k_newest.new_empty(shape)
+
+
+@torch.library.custom_op("b200::kv8_attention", mutates_args=(), device_types="cuda")
+def kv8_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale: Tensor, v_scale: Tensor, k_newest: Tensor,
+                  v_newest: Tensor, table: Tensor, rows: Optional[Tensor], cu: Tensor, lens: Tensor, max_q_len: int,
+                  scale: Optional[float]) -> Tensor:
+    """serving.PagedKV8.attend on the cache's tensors."""
+    cache = serving.PagedKV8(k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows)
+    return cache.attend(q, cu, lens, max_q_len=max_q_len, scale=scale)
+
+
+@kv8_attention.register_fake
+def _kv8_attention_fake(q, k_pages, v_pages, k_scale, v_scale, k_newest, v_newest, table, rows, cu, lens, max_q_len, scale):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -591,6 +591,26 @@ def test_decoder_follows_the_model(sv, tt):
         assert ((y - want[0, :10]).norm() / want[0, :10].norm()).item() < 0.05
 
 
+def test_ops_compiled_match_the_calls(sv):
+    """A step written with torch.ops.b200, compiled with fullgraph=True, equals the calls."""
+    m, n = (Model(sv, 2, 2, 64, 16, 64, torch.float16, seed=9) for _ in range(2))
+    x = torch.randn(6, 128, device="cuda").half()
+    w, ws = sv.quantize_weight(torch.randn(8 * 64, 128, device="cuda") / 11)
+    cu, start, lens = starts([3, 3]), i32([0, 0]), i32([3, 3])
+    ops = torch.ops.b200
+
+    def step(x):
+        qkv = ops.linear_int8(x, w, ws, None, False, None, False)
+        q = ops.kv8_append(qkv, *m.c.tensors, cu, start, 4, None, None, False)
+        return ops.kv8_attention(q, *m.c.tensors, cu, lens, 3, None), *ops.kv8_read(*m.c.tensors, cu, start, lens, 6)
+
+    got = torch.compile(step, fullgraph=True)(x)
+    q = n.c.append(sv.linear_int8(x, w, ws), cu, start, heads=4)
+    want = (n.c.attend(q, cu, lens, max_q_len=3), *n.c.read(cu, start, lens, total=6))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals(sv):
     m = Model(sv, 2, 2, 64, 16, 64, torch.float16)

@@ -113,3 +113,25 @@ def test_cpu_tensors_are_refused(pkg):
         sv.linear_int8(torch.randn(2, 16), torch.zeros(4, 16, dtype=torch.int8), torch.ones(4))
     with pytest.raises(ValueError):
         sv.PagedKV8.allocate(8, 2, 48, 64, table)
+
+
+def test_ops_fake_shapes(pkg):
+    """torch.ops.b200's serving ops under a fake mode (what torch.compile traces with)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = torch.ops.b200
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.float16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        x, w, ws = t(5, 100), t(40, 112, dtype=torch.int8), t(40, dtype=torch.float32)
+        assert ops.linear_int8(x, w, ws, None, True, None, False).shape == (5, 40)
+        assert ops.linear_int8(x, w, ws, None, False, t(5, 40, dtype=torch.float32), False).dtype == torch.float32
+        u8, f32, i32 = torch.uint8, torch.float32, torch.int32
+        cache = (t(9, 2, 16, 64, dtype=u8), t(9, 2, 4, 64, 4, dtype=u8), t(9, 2, dtype=f32), t(9, 2, dtype=f32),
+                 t(3, 2, 2, 16, 64), t(3, 2, 2, 4, 64, 4), t(3, 3, dtype=i32), None)
+        cu, at = t(4, dtype=i32), t(3, dtype=i32)
+        q = ops.kv8_append(t(7, 8 * 64), *cache, cu, at, 4, None, None, False)
+        assert q.shape == (7, 4, 64) and q.dtype == torch.float16
+        k, v = ops.kv8_read(*cache, cu, at, at, 11)
+        assert k.shape == v.shape == (11, 2, 64)
+        assert ops.kv8_attention(q, *cache, cu, at, 3, None).shape == q.shape
