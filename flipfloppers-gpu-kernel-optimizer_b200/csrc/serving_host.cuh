@@ -163,9 +163,14 @@ int launch_attn8_tile(Attn8Params& p, long long rows, cudaStream_t st) {
   return launch_status();
 }
 
-// Whether the 256-row tcgen05 kernel is ahead of the warps' streams: rows (new tokens times the group) in all.
+// Whether the 256-row tcgen05 kernel is ahead of the warps' streams.  Its time goes by the waves of 256-row items
+// over the SMs, theirs by the rows (new tokens times query heads); a wave takes as long as this many rows.  Measured
+// (warps against tiles, us): 8192 rows over 8000 keys, D = 128: 222, 212; D = 64: 147, 165; D = 32: 117, 145;
+// 16384 rows, D = 128: 425, 215; D = 64: 274, 166; 8 x 256 rows of 16 heads over 2000 keys, D = 32: 122, 49; 4096
+// rows of D = 128: 123, 213.
 bool attn8_many_rows(long long rows, int kv_heads, int batch, int head_dim) {
-  return rows / batch >= 128 && rows * kv_heads * head_dim >= 300000;
+  const long long items = (rows / batch + 255) / 256 * batch * kv_heads, waves = (items + num_sms() - 1) / num_sms();
+  return rows * kv_heads >= waves * (head_dim == 128 ? 8000 : 10000);
 }
 
 template <int D>

@@ -361,7 +361,9 @@ int b200_kv8_read(const B200KvCache8* cache, const int* cu, const int* start, co
  * [tokens, heads, head_dim] is the token at position lens[b] - n + i of sequence b
  * (n = cu[b+1] - cu[b] new tokens, all appended already), which sees the keys up
  * to its own; heads % kv_heads == 0, consecutive query heads share a key head.  A
- * row with no key (position < 0) gives zeros.  max_q_len >= every n.  No atomics:
+ * row with no key (position < 0) gives zeros.  What is not finite in the newest block
+ * reaches the rows that see it and no others (NaN, or the infinity in its channel).
+ * max_q_len >= every n.  No atomics:
  * the same inputs give the same bits. */
 size_t b200_kv8_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int max_q_len);
 int b200_kv8_attention(const B200KvCache8* cache, const void* q, long long ld_q, void* out, long long ld_out,

@@ -313,7 +313,7 @@ def test_attend_many_chunks_of_rows(sv):
     m.check_attend(q, [2500, 1500, 1300, 1], 16)
 
 
-PROMPTS = [  # page, dim, kv, group, lens before, new tokens: enough rows for the 256-row kernel
+PROMPTS = [  # page, dim, kv, group, lens before, new tokens: about as many rows as the 256-row kernel takes, and more
     (64, 64, 8, 1, [0, 129], [640, 257]),
     (128, 128, 4, 2, [1000, 0], [300, 511]),
     (16, 32, 8, 3, [7, 300], [401, 255]),
@@ -321,6 +321,11 @@ PROMPTS = [  # page, dim, kv, group, lens before, new tokens: enough rows for th
     (16, 64, 16, 1, [0, 0, 33], [1, 385, 700]),
     (128, 32, 8, 8, [4000], [200]),
     (32, 64, 4, 4, [31, 500], [333, 0]),
+    (64, 64, 8, 1, [0, 129], [1000, 513]),
+    (128, 128, 4, 2, [1000, 0], [700, 511]),
+    (32, 128, 2, 5, [63], [901]),
+    (16, 64, 4, 4, [31, 500], [700, 0]),
+    (64, 32, 16, 1, [0, 257], [900, 3]),
 ]
 
 
@@ -328,7 +333,7 @@ PROMPTS = [  # page, dim, kv, group, lens before, new tokens: enough rows for th
 @pytest.mark.parametrize("case", range(len(PROMPTS)))
 def test_attend_prompts(sv, pkg, case, dtype):
     page, dim, kv, group, before, new = PROMPTS[case]
-    assert sum(new) * group // len(new) >= 128 and sum(new) * group * kv * dim >= 300000  # the launcher's rule
+    assert sum(new) * group // len(new) >= 128 and sum(new) * group * kv * dim >= 300000
     m = Model(sv, len(before), kv, dim, page, max(a + b for a, b in zip(before, new)), dtype, seed=50 + case)
     if sum(before):
         m.append(before, kv * group)
@@ -338,41 +343,49 @@ def test_attend_prompts(sv, pkg, case, dtype):
     assert pkg.runtime.device_error() == 0
 
 
-def test_prompt_rows_without_keys(sv):
+@pytest.mark.parametrize("kv", [8, 16])  # the warps' kernel, and the 256-row kernel
+def test_prompt_rows_without_keys(sv, kv):
     """More new rows than cached tokens: the first rows see nothing."""
-    m = Model(sv, 2, 8, 64, 16, 512, torch.float16)
-    m.append([300, 0], 8)
-    q = m.rows(1200, 8 * 64).view(1200, 8, 64)
-    out = m.check_attend(q, [600, 600], 8)
+    m = Model(sv, 2, kv, 64, 16, 512, torch.float16)
+    m.append([300, 0], kv)
+    q = m.rows(1200, kv * 64).view(1200, kv, 64)
+    out = m.check_attend(q, [600, 600], kv)
     assert not bool(out[:300].any()) and not bool(out[600:].any())
 
 
+@pytest.mark.parametrize("kv", [8, 16])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
-def test_prompt_scales_far_apart(sv, dtype):
-    """Blocks of very different sizes and of zeros, rows of any size, in the 256-row kernel."""
-    m = Model(sv, 1, 8, 64, 32, 1024, dtype)
-    x = m.rows(1000, 24 * 64)
-    x[:, 1024:] *= (torch.arange(1000, device="cuda") // 32 % 5).to(dtype)[:, None] * 0.25
-    x[128:256, 512:] *= 2 ** -6
-    x[256:288, 512:] = 0
-    x[:32, 1024:] = 0
-    x[990:, 1024:] *= 2 ** -5
-    q = m.append([1000], 8, qkv=x)
-    m.check_attend(q, [1000], 8)
+def test_prompt_scales_far_apart(sv, dtype, kv):
+    """Blocks of very different sizes and of zeros."""
+    m = Model(sv, 1, kv, 64, 32, 1024, dtype)
+    k, v = kv * 64, 2 * kv * 64
+    x = m.rows(1000, 3 * kv * 64)
+    x[:, v:] *= (torch.arange(1000, device="cuda") // 32 % 5).to(dtype)[:, None] * 0.25
+    x[128:256, k:] *= 2 ** -6
+    x[256:288, k:] = 0
+    x[:32, v:] = 0
+    x[990:, v:] *= 2 ** -5
+    q = m.append([1000], kv, qkv=x)
+    m.check_attend(q, [1000], kv)
+    if dtype == torch.float16:
+        m.check_attend(q, [1000], kv, scale=-0.05)  # a factor that is not positive
 
 
-def test_prompt_nan_stays_with_the_rows_that_see_it(sv):
-    m = Model(sv, 1, 8, 64, 64, 1024, torch.float16)
-    x = m.rows(1000, 24 * 64)
+@pytest.mark.parametrize("kv", [8, 16])
+def test_prompt_nan_stays_with_the_rows_that_see_it(sv, kv):
+    m = Model(sv, 1, kv, 64, 64, 1024, torch.float16)
+    k, v = kv * 64, 2 * kv * 64
+    x = m.rows(1000, 3 * kv * 64)
     clean = x.clone()
-    x[400, 1024 + 7] = float("nan")  # a value of head 0: block 6 is NaN as a whole
-    x[990, 1024 + 70] = float("inf")  # a value of head 1 in the newest block
-    x[980, 512 + 128] = float("nan")  # a key of head 2 in the newest block
-    out = m.c.attend(m.c.append(x, starts([1000]), i32([0]), heads=8), starts([1000]), i32([1000]), max_q_len=1000)
-    q = m.append([1000], 8, qkv=clean, start=[0])
-    want = m.check_attend(q, [1000], 8)
+    x[400, v + 7] = float("nan")  # a value of head 0: block 6 is NaN as a whole
+    x[990, v + 70] = float("inf")  # a value of head 1 in the newest block
+    x[980, k + 128] = float("nan")  # a key of head 2 in the newest block
+    out = m.c.attend(m.c.append(x, starts([1000]), i32([0]), heads=kv), starts([1000]), i32([1000]), max_q_len=1000)
+    q = m.append([1000], kv, qkv=clean, start=[0])
+    want = m.check_attend(q, [1000], kv)
     assert torch.equal(out[:384, 0], want[:384, 0]) and bool(out[384:, 0].isnan().all())
-    assert torch.equal(out[:990, 1], want[:990, 1]) and not bool(out[990:, 1].isfinite().any())
+    # (the channel it is in; the 256-row kernel gives NaN to all channels of a row that sees it)
+    assert torch.equal(out[:990, 1], want[:990, 1]) and not bool(out[990:, 1, 6].isfinite().any())
     assert torch.equal(out[:980, 2], want[:980, 2]) and bool(out[980:, 2].isnan().all())
     assert torch.equal(out[:, 3:], want[:, 3:])
 
