@@ -297,6 +297,28 @@ def test_attend(sv, pkg, case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attend_in_a_wide_table(sv, case, dtype):
+    """The same where the table could hold long sequences: the work is then one line cut among all warps."""
+    page, dim, kv, group, before, new = CASES[case]
+    m = Model(sv, len(before), kv, dim, page, 9000, dtype, seed=case + 20, rows=case % 2 == 0)
+    if sum(before):
+        m.append(before, kv * group)
+    q = m.append(new, kv * group)
+    a = m.check_attend(q, new, kv * group)
+    assert torch.equal(a, m.check_attend(q, new, kv * group))
+
+
+def test_attend_ragged_in_a_wide_table(sv):
+    """Many sequences, short and long: pieces that hold ends and starts of several."""
+    m = Model(sv, 40, 4, 64, 16, 5000, torch.float16, seed=4)
+    before = [(i * 997) % 1300 if i % 3 else i for i in range(39)] + [4990]
+    m.append(before, 8)
+    q = m.append([1 + i % 3 for i in range(40)], 8)
+    m.check_attend(q, [1 + i % 3 for i in range(40)], 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
 def test_attend_long(sv, dtype):
     """A long sequence beside short ones: its keys are cut among many warps."""
     m = Model(sv, 3, 2, 64, 64, 40000, dtype)
