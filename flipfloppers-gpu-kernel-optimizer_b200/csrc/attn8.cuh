@@ -34,7 +34,6 @@ namespace b200 {
 constexpr int ATTN8_CHUNK = 32;   // tokens
 // Weights are kept times 2^14 (at most 16384), so that fp16 has eleven bits for those down to 2^-28 of the largest.
 constexpr float ATTN8_LIFT = 14.f;
-enum Attn8Mode : int { ATTN8_LINE = 0, ATTN8_CTA = 1, ATTN8_WARP = 2 };
 constexpr int ATTN8_MAX_BATCH = 2048;
 
 struct Attn8Params {
@@ -45,8 +44,6 @@ struct Attn8Params {
   const int* cu;         // [batch + 1] first row of each sequence's new tokens
   const int* lens;       // [batch] cached tokens, the new ones included
   int tokens, batch, heads;
-  int mode;              // ATTN8_LINE: the line of units cut into equal pieces; ATTN8_CTA: a row tile a CTA, cut among
-                         // its warps; ATTN8_WARP: a row tile a warp
   float scale_log2;      // scale * log2(e)
   int warps;             // warps of the launch
   int* plan;             // [batch + 1] first unit of each sequence on the line (written by CTA 0)
@@ -686,7 +683,8 @@ __device__ __forceinline__ void attn8_sequence(const Attn8Params& p, int b, int&
   }
 }
 
-template <int D, int NT, bool SMALL>
+// OWN: a row tile a CTA, cut among its warps; else the line of units, cut among all warps.
+template <int D, int NT, bool SMALL, bool OWN>
 __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const Attn8Params p) {
   using C = Attn8Cfg<D, NT>;
   extern __shared__ __align__(128) uint8_t smem_attn8[];
@@ -705,7 +703,7 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
     if (b < p.batch) {
       int t0, q_len, len;
       attn8_sequence(p, b, t0, q_len, len);
-      n = p.c.kv_heads * ((q_len * group + C::ROWS - 1) / C::ROWS) * (p.mode == ATTN8_LINE ? attn8_units(len, p.c.page) : 1);
+      n = p.c.kv_heads * ((q_len * group + C::ROWS - 1) / C::ROWS) * (OWN ? 1 : attn8_units(len, p.c.page));
     }
     int sum = n;
 #pragma unroll
@@ -725,7 +723,7 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
   }
   if (tid == 0) line[p.batch] = base;
   __syncthreads();
-  if (p.mode == ATTN8_LINE && blockIdx.x == 0)
+  if (!OWN && blockIdx.x == 0)
     for (int i = tid; i <= p.batch; i += 32 * C::WARPS) p.plan[i] = line[i];
 
   Attn8Warp<D, NT, SMALL> w(p, smem_attn8, wid);
@@ -736,7 +734,7 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
     int t0, q_len, len;
     attn8_sequence(p, b, t0, q_len, len);
     const int tiles = (q_len * group + C::ROWS - 1) / C::ROWS;
-    units = p.mode == ATTN8_LINE ? attn8_units(len, p.c.page) : 1;
+    units = OWN ? 1 : attn8_units(len, p.c.page);
     const int item = (at - line[b]) / units;
     u0 = (at - line[b]) % units;
     w.s.b = b;
@@ -766,17 +764,7 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
     return make_float2(top, sum);
   };
 
-  if (p.mode == ATTN8_WARP) {
-    for (int at = warp; w.ok && at < base; at += p.warps) {
-      int units, u0;
-      locate(at, units, u0);
-      w.load_rows();
-      w.stream(0, attn8_chunks(w.s.len, p.c.page));
-      w.finish();
-    }
-    return;
-  }
-  if (p.mode == ATTN8_CTA) {
+  if constexpr (OWN) {
     for (int at = blockIdx.x; at < base; at += gridDim.x) {  // (the barriers are reached whatever a wait did)
       int units, u0;
       locate(at, units, u0);

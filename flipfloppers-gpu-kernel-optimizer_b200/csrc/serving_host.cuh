@@ -135,26 +135,22 @@ int launch_attn8(Attn8Params& p, long long rows, cudaStream_t st) {
   const int ctas = std::min(num_sms(), 150);  // (the join kernel holds a part a CTA)
   p.warps = ctas * C::WARPS;
   p.plan = reinterpret_cast<int*>(p.part + ctas * attn8_slots<D, NT>());
-  // Whole row tiles keep every warp busy when there are several a warp; else the keys are cut too.  Few tiles of
-  // short tables (at most four chunks a warp of a CTA) are a CTA's each, which adds up its parts itself: no second
-  // kernel.  Measured (line against CTA, us on the device, one token a sequence): 1 x 1000 keys of 16 heads of 64: 12.1,
-  // 8.4; 8 x 2000: 18.0, 11.2; 16 x 1000 (288 tiles): 19.5, 15.5; 16 x 1000 keys of 32/8 heads of 128: 19.1, 11.1; past
-  // the bounds 1 x 4000: 13.2, 16.5; 32 x 1000 (576 tiles): 26.2, 28.9; 4 x 3000 of 32/8 heads: 17.3, 20.0.
+  // Few tiles of short tables (at most four chunks a warp of a CTA) are a CTA's each, which adds up its parts itself:
+  // no second kernel.  Measured (line against CTA, us on the device, one token a sequence): 1 x 1000 keys of 16 heads of
+  // 64: 12.1, 8.4; 8 x 2000: 18.0, 11.2; 16 x 1000 (288 tiles): 19.5, 15.5; 16 x 1000 keys of 32/8 heads of 128: 19.1,
+  // 11.1; past the bounds 1 x 4000: 13.2, 16.5; 32 x 1000 (576 tiles): 26.2, 28.9; 4 x 3000 of 32/8 heads: 17.3, 20.0.
   const long long tiles = (rows / C::ROWS + p.batch) * p.c.kv_heads;
-  const long long chunks = static_cast<long long>(p.c.table_width) * p.c.page / ATTN8_CHUNK;
-  p.mode = rows / C::ROWS * p.c.kv_heads >= 4LL * p.warps ? ATTN8_WARP
-           : tiles <= 2 * ctas && chunks <= 4 * C::WARPS ? ATTN8_CTA : ATTN8_LINE;
-  auto kern = k_attn8<D, NT, SMALL>;
+  const bool own = tiles <= 2 * ctas && static_cast<long long>(p.c.table_width) * p.c.page / ATTN8_CHUNK <= 4 * C::WARPS;
   static_assert(C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4 + 128 <= 227 * 1024, "ring and line fit an SM");
+  auto kern = own ? k_attn8<D, NT, SMALL, true> : k_attn8<D, NT, SMALL, false>;
   if (int rc = set_smem(reinterpret_cast<const void*>(kern), C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4)) return rc;
-  launch_kernel(kern, dim3(ctas), dim3(32 * C::WARPS), C::TOTAL + (p.batch + 1) * 4, st, p);
+  launch_kernel(kern, dim3(own ? static_cast<unsigned>(std::min<long long>(tiles, ctas)) : ctas), dim3(32 * C::WARPS),
+                C::TOTAL + (p.batch + 1) * 4, st, p);
   if (int rc = launch_status()) return rc;
-  if (p.mode == ATTN8_LINE) {
-    launch_kernel(k_attn8_join<D, NT>, dim3(static_cast<unsigned>(rows / C::ROWS + p.batch), p.c.kv_heads),
-                  dim3(ATTN8_JOIN_THREADS), 0, st, p);
-    return launch_status();
-  }
-  return B200_OK;
+  if (own) return B200_OK;
+  launch_kernel(k_attn8_join<D, NT>, dim3(static_cast<unsigned>(rows / C::ROWS + p.batch), p.c.kv_heads),
+                dim3(ATTN8_JOIN_THREADS), 0, st, p);
+  return launch_status();
 }
 
 template <int D>
@@ -254,7 +250,8 @@ int quantize_rows_impl(const void* x, int x_type, long long ld_x, void* codes, l
                   m, k, vec);
     return launch_status();
   };
-  if (k <= 2048) {
+  // a warp a row where that makes CTAs enough, else a CTA a row
+  if (k <= 2048 && m >= 2048) {
     if (x_type == DT_F16) return run(k_quant_rows<DT_F16, 32>, 8);
     if (x_type == DT_BF16) return run(k_quant_rows<DT_BF16, 32>, 8);
     return run(k_quant_rows<DT_F32, 32>, 8);

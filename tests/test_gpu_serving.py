@@ -328,7 +328,7 @@ def test_attend_long(sv, dtype):
 
 
 def test_attend_many_chunks_of_rows(sv):
-    """Enough row tiles that every warp takes whole ones."""
+    """Prompts of several sequences, and one new token beside them."""
     m = Model(sv, 4, 8, 64, 64, 2500, torch.float16)
     m.append([0, 100, 1200, 64], 16)
     q = m.append([2500, 1500, 1300, 1], 16)
