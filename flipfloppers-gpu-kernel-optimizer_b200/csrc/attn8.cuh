@@ -20,8 +20,8 @@
 //     codes are widened to fp16 (exactly: 1024 + c, less 1152) once for all rows;
 //   - scores take the block's K scale, and each block's V product its V scale, in
 //     fp32: the codes enter the products as whole numbers.
-// Measured: 64 sequences of 1 to 8191 tokens, 32/8 heads of 128, 103 us (5.0 TB/s); one of
-// 131000 tokens 60 us (4.4 TB/s, 41 to 45 us of it streaming).
+// Measured: 64 sequences of 1 to 8191 tokens, 32/8 heads of 128, 98 us (5.3 TB/s); one of
+// 131000 tokens 58 us (4.6 TB/s, 41 to 45 us of it streaming).
 // Contraction order is free, so a lane's 16 bytes of K are the fragment elements of
 // four steps; key tau(m) = 4 (m/2) + m%2 (+2 for m >= 8) sits in row m, which after
 // the 8x8 transposition of P (movmatrix) meets the word of V with the same four keys.

@@ -16,7 +16,7 @@
 // of the token's largest value); a token whose V has an infinity or NaN gives NaN to the
 // rows that see it and nothing to the others.
 // Bound: the softmax (the exponentials alone, 16 a clock and SM, take 2048 clocks for two 128x128 tiles; a row's 128
-// weights take its one thread about 2500).  Measured: 2048 tokens over 17200 keys, 16 heads of 64, 347 us (392 TFLOP/s);
+// weights take its one thread about 2500).  Measured: 2048 tokens over 17200 keys, 16 heads of 64, 343 us (397 TFLOP/s);
 // 1024 tokens over 8000 keys, 32/8 heads of 128, 255 us.
 #pragma once
 

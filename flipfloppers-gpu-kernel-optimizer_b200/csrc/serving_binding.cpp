@@ -286,7 +286,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 int type_code(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
 
-// linear(x, w, w_scale, bias, gelu, resid, out_dtype or None, out or None) -> out
+// linear_i8(x, w, w_scale, bias, gelu, resid, out_dtype or None, out or None) -> out
 PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count(n, 8)) return nullptr;
   return guarded([&]() -> PyObject* {
@@ -365,7 +365,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 PyMethodDef methods[] = {{"cache", FAST(py_cache), nullptr},   {"append", FAST(py_append), nullptr},
                          {"read", FAST(py_read), nullptr},     {"attend", FAST(py_attend), nullptr},
-                         {"linear", FAST(py_linear), nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         {"linear_i8", FAST(py_linear), nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200serving", "8-bit serving operators", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

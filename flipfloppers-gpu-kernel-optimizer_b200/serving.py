@@ -166,7 +166,7 @@ def linear_int8(x: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = 
     of 16, at least k (``quantize_weight``); ``w_scale`` and ``bias`` fp32 [n].  With ``gelu`` the
     exact GELU follows.  ``resid`` fp32 [m, n] is added last: the result is fp32, and ``out`` may be
     ``resid`` itself.  Without it the result has ``out_dtype`` (default: x's type)."""
-    return _done(_native().linear(x, w, w_scale, bias, gelu, resid, out_dtype, out), "b200_linear_i8")
+    return _done(_native().linear_i8(x, w, w_scale, bias, gelu, resid, out_dtype, out), "b200_linear_i8")
 
 
 # ------------------------------------------------------------------ a block stack served in 8 bits
