@@ -789,6 +789,7 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
         *reinterpret_cast<uint2*>(p.out + (w.s.t0 + tok) * p.ld_out +
                                   static_cast<size_t>(w.s.head * group + (row0 + r) % group) * D + d) = out;
       }
+      fence_proxy_async_smem();  // the next tile's copies overwrite the parts
       __syncthreads();
     }
     return;

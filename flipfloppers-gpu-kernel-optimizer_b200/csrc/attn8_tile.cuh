@@ -201,6 +201,11 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   griddep_sync();
   int items = 0;
   for (int b0 = 0; b0 < p.batch; b0 += C::THREADS) {
@@ -227,11 +232,6 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
     if (b < p.batch) line[b] = before + sum - n;
     __syncthreads();
   }
-  tc_fence_before();
-  __syncwarp();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
   const int G = gridDim.x;
 
   if (warp == 0) {
