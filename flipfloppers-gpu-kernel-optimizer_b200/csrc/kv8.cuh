@@ -326,10 +326,13 @@ __device__ __forceinline__ void kv8_append_head(const Kv8AppendParams& p, int wh
 
 // Unit = one touched block of one sequence.  blockIdx.x: unit (or token, by_token);
 // blockIdx.y: k_each heads of K, a head of V, or q_each query heads.
-// Memory-bound.  Measured: 18400 tokens of 16 + 2 x 16 heads of 64 in 51 us (3.7 TB/s), 128 single tokens of 32/8 heads
-// of 128 in 10 us (the blocks that become whole: chains of dependent loads).  Heads of one CTA share the rows of cos and sin through L1 (with a head a CTA they came from L2 for
-// every head, twice the bytes of the head itself: 114 us against 77 us for 27000 tokens of 16 + 2 x 16 heads).  Shared memory holds the block's 16-bit values, in the order of the page's codes, between the
-// maximum and the codes, so that nothing is read twice.
+// Memory-bound.  Measured: 18400 tokens of 16 + 2 x 16 heads of 64 in 51 us (3.7 TB/s),
+// 128 single tokens of 32/8 heads of 128 in 10 us (the blocks that become whole: chains of
+// dependent loads).  Heads of one CTA share the rows of cos and sin through L1 (with a head
+// a CTA they came from L2 for every head, twice the bytes of the head itself: 114 us against
+// 77 us for 27000 tokens of 16 + 2 x 16 heads).  Shared memory holds the block's 16-bit
+// values, in the order of the page's codes, between the maximum and the codes, so that
+// nothing is read twice.  Four CTAs an SM (64 registers): with three it took 59 us.
 template <bool BF16>
 __global__ void __launch_bounds__(256, 4) k_kv8_append(const Kv8AppendParams p) {
   extern __shared__ uint4 smem_kv8[];
@@ -407,8 +410,9 @@ struct Kv8ReadParams {
   int tokens, batch;
 };
 
-// Windows of tokens as 16-bit rows (18400 tokens of 16 heads of 64 in 27 us, 4.2 TB/s).  A warp takes four tokens of one head: lanes
-// run along the channels, eight a lane, so rows leave in 16-byte stores.
+// Windows of tokens as 16-bit rows (18400 tokens of 16 heads of 64 in 26 us, 4.3 TB/s).
+// Lanes run along the channels, eight a lane, so rows leave in 16-byte stores: a warp takes
+// 8, 4 or 2 tokens of one head (head_dim 32, 64, 128).
 template <bool BF16>
 __global__ void __launch_bounds__(256) k_kv8_read(const Kv8ReadParams p) {
   griddep_sync();
