@@ -11,7 +11,7 @@
 // is not full is read from there; it is quantized once, from its 16-bit values,
 // when its last token arrives.  So what the cache holds does not depend on how
 // the tokens were split among calls, and a sequence may be shortened to any
-// length its newest two blocks still reach (drafted tokens that were refused).
+// length that the two blocks written last still reach (drafted tokens that were refused).
 //
 // Arithmetic: rotation in fp32 with separately rounded products, then one
 // rounding to 16 bits; scale = amax * (1/127); code = rint(x / scale), clamped to

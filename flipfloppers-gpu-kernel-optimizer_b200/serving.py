@@ -77,7 +77,9 @@ class PagedKV8:
 
     A block is quantized once, when its last token arrives, so the cache does not depend on how
     tokens were split among calls.  Appending at an earlier start shortens a sequence first; that
-    may go back to the first token of its newest two blocks."""
+    may go back to the first token of the newest two blocks it has had since it was empty (a slot
+    keeps the latest block that was written to it: shortening a sequence does not bring back the
+    block before)."""
 
     def __init__(self, k_pages: Tensor, v_pages: Tensor, k_scale: Tensor, v_scale: Tensor, k_newest: Tensor,
                  v_newest: Tensor, table: Tensor, rows: Optional[Tensor] = None):
@@ -175,8 +177,8 @@ class Int8Decoder:
 
     ``open()`` gives a sequence id; ``forward(x, seqs, counts)`` appends counts[i] tokens to sequence
     seqs[i] and returns their outputs: a prompt, a chunk of one, drafted tokens or one token a
-    sequence, mixed at will.  ``rewind(seq, n)`` drops the last n tokens (of the newest two blocks),
-    ``close(seq)`` frees a sequence's pages.  ``rope_base`` turns on the position rotation (the
+    sequence, mixed at will.  ``rewind(seq, n)`` drops the last n tokens (of the newest two blocks
+    that the sequence has had, as far as PagedKV8 keeps them), ``close(seq)`` frees a sequence's pages.  ``rope_base`` turns on the position rotation (the
     model itself has none: its inputs carry their positions).  Head dims 32, 64 and 128."""
 
     def __init__(self, model, max_sequences: int, max_tokens: int, page_size: int = 64,
@@ -209,13 +211,14 @@ class Int8Decoder:
                 -torch.arange(0, hd, 2, device=self.dev, dtype=torch.float64) / hd)
             self.cos, self.sin = turn.cos().float(), turn.sin().float()
         self.lens = [-1] * max_sequences  # -1: not open
+        self.kept = [0] * max_sequences   # first token that the slots of the newest blocks still hold
         self.pages: List[List[int]] = [[] for _ in range(max_sequences)]
         self.spare = list(range(pages - 1, -1, -1))
 
     def open(self) -> int:
         seq = self.lens.index(-1) if -1 in self.lens else -1
         _need(seq >= 0, "every sequence is in use")
-        self.lens[seq] = 0
+        self.lens[seq] = self.kept[seq] = 0
         return seq
 
     def close(self, seq: int) -> None:
@@ -225,10 +228,10 @@ class Int8Decoder:
 
     def rewind(self, seq: int, n: int) -> None:
         """Drop the last n tokens of a sequence."""
-        length, p = self.lens[seq], self.page_size
+        length = self.lens[seq]
         _need(length >= 0, f"sequence {seq} is not open")
-        _need(0 <= n <= length and (n == 0 or length - n >= max(0, (length - 1) // p - 1) * p),
-              "rewind reaches back to the first token of the newest two blocks")
+        _need(0 <= n <= length and (n == 0 or length - n >= self.kept[seq]),
+              "rewind reaches back to the first token of the newest two blocks the sequence has had")
         self.lens[seq] = length - n
 
     def forward(self, x: Tensor, seqs: Sequence[int], counts: Sequence[int]) -> Tensor:
@@ -248,6 +251,7 @@ class Int8Decoder:
         new = [0] * n
         for s, c in zip(seqs, counts):
             new[s] = c
+            self.kept[s] = max(self.kept[s], ((self.lens[s] + c - 1) // p - 1) * p)
             grown = []
             while len(self.pages[s]) * p < self.lens[s] + c:
                 self.pages[s].append(self.spare.pop())

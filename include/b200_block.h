@@ -323,7 +323,8 @@ int b200_block_forward_noalloc(const B200BlockArgs* args, b200_stream_t stream);
  * that is not full is read from there; when its last token arrives it is
  * quantized from its 16-bit values (scale = largest magnitude / 127; a block with
  * an infinity or NaN gets a NaN scale).  A sequence may be shortened by starting
- * the next append earlier, down to the first token of its newest two blocks.
+ * the next append earlier, down to the first token of the newest two blocks that it
+ * has had since it was empty (a slot keeps the latest block written to it).
  * table [batch][table_width]: the page of each block of each sequence.
  * head_dim 32, 64 or 128; page_size 16, 32, 64 or 128; batch <= 2048.  All on the
  * device, 16-byte aligned.  A page, row or length outside its buffer is skipped
