@@ -11,7 +11,10 @@
 //                works for the other.
 // Scales: with w = s + log2(V scale), P = 2^(w - max w + 14) carries a key's V scale (P <= 2^14,
 // and O needs no scale of its own), and the softmax's sum takes P / (V scale).  K's scale
-// multiplies the score.  A block of zeros counts as scale 2^-100.  The newest block's
+// multiplies the score.  A tile with a V of zeros, or with V scales outside 2^-40 .. 2^40, is `far`: there
+// P / (V scale) could leave fp32's range on either side (a scale of 2^-100 and 16384 keys make 2^14 * 2^100 * 2^14).
+// From the first such tile of an item on, the sum takes exponentials of the scores themselves, twice as many, with a
+// reference of its own, and V of zeros weighs nothing in the products.  The newest block's
 // 16-bit values are brought into fp16 by a power of two for each token (exact to 2^-24
 // of the token's largest value); a token whose V has an infinity or NaN gives NaN to the
 // rows that see it and nothing to the others.
@@ -38,7 +41,8 @@ struct Attn8TileCfg {
   static constexpr int OFF_KV = 2 * Q_BYTES;         // stage s: K, then V
   static constexpr int OFF_KEY = OFF_KV + ST * 2 * KV_BYTES;        // [ST][3][BN]: K factor, log2 V scale, 1 / V scale
   static constexpr int OFF_QF = OFF_KEY + ST * 3 * BN * 4;          // [2][ROWS] row factors, by item parity
-  static constexpr int OFF_BAR = OFF_QF + 2 * ROWS * 4;
+  static constexpr int OFF_AHEAD = OFF_QF + 2 * ROWS * 4;           // [ROWS] see attn8_weights_far
+  static constexpr int OFF_BAR = OFF_AHEAD + ROWS * 4;
   static constexpr int TOTAL = OFF_BAR + 256;        // + line + alignment
   // tensor memory: S/P of the tiles at 0 and 128, O at 256 and 256 + D
   static constexpr uint32_t TM_O = 256;
@@ -163,6 +167,47 @@ __device__ __forceinline__ void attn8_weights_each(float (&s)[128], const float*
   l = l * alpha + sum;
 }
 
+// The same where V scales may be anything (log2 of the V scale is -inf for zeros): l is relative to
+// 2^(m - ATTN8_LIFT + *ahead), *ahead >= 0 (0 before the row's first such tile).  The scores are read twice from tensor
+// memory at `ts`, 64 at a time, and the weights written over those that have been read.  Returns (m, l, alpha).  In a
+// loop of its own after the ordinary tiles' loop: as a branch within that it took the 17200-key chunk from 338 to 360 us.
+__device__ __forceinline__ float3 attn8_weights_far(uint32_t ts, const float* key, float qf, int k0, int lim, float m, float l,
+                                                 float* ahead, bool first) {
+  float now = m, most = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < 128; h += 64) {
+    float s[64];
+    tmem_ld64(ts + h, s);
+#pragma unroll
+    for (int c = 0; c < 64; ++c) {
+      const float x = k0 + h + c < lim ? s[c] * (key[h + c] * qf) : -INFINITY;
+      most = fmaxf(most, x);
+      now = fmaxf(now, k0 + h + c < lim ? x + key[128 + h + c] : -INFINITY);
+    }
+  }
+  const float lwas = m - ATTN8_LIFT + (first ? 0.f : *ahead), lref = fmaxf(lwas, most), base = lref == -INFINITY ? 0.f : lref;
+  if (now == -INFINITY) now = lref - 200.f;  // zeros only so far: a reference below that of any scale that can follow
+  const float top = now == -INFINITY ? 0.f : now, ref = top - ATTN8_LIFT;  // (no key seen yet: every weight is 0)
+  float sum = 0.f;
+#pragma unroll 1
+  for (int h = 0; h < 128; h += 64) {
+    float s[64], p[32];
+    tmem_ld64(ts + h, s);
+#pragma unroll
+    for (int c = 0; c < 64; ++c) {
+      const float x = k0 + h + c < lim ? s[c] * (key[h + c] * qf) : -INFINITY;
+      sum += fast_exp2(x - base);
+      s[c] = k0 + h + c < lim ? fast_exp2(x + (key[128 + h + c] - ref)) : 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < 32; ++c) p[c] = __uint_as_float(pack_half2(s[2 * c], s[2 * c + 1]));
+    tmem_st32(ts + h / 2, p);
+  }
+  const float over = lref - ref;
+  *ahead = fmaxf(0.f, over);
+  return make_float3(now, (l * fast_exp2(lwas - base) + sum) * fast_exp2(fminf(0.f, over)), fast_exp2(m - top));
+}
+
 template <int D>
 __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(const Attn8Params p) {
   using C = Attn8TileCfg<D>;
@@ -180,6 +225,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
   uint64_t* drain = bars + 12;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* far = reinterpret_cast<int*>(tmem_slot + 2);  // [ST] of the stage's tile: its number plus 1 if it is a far one
   int* line = reinterpret_cast<int*>(smem + C::TOTAL);  // [batch + 1] first item of each sequence
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.heads / p.c.kv_heads;
@@ -194,7 +240,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
       mbar_init(&o_done[i], 1);
     }
     mbar_init(drain, 1);
-    *abort_flag = 0;
+    *abort_flag = far[0] = far[1] = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -428,10 +474,11 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         for (int n = 0; n < 2; ++n) {
           const int kt = i + C::CONV * n;
           if (kt < min(limit, 128)) {
-            const float v = vsc[n] < 7.8886091e-31f ? 7.8886091e-31f : vsc[n];  // 2^-100 at least; NaN stays
+            const float v = vsc[n];
             key[kt] = ksc[n];
-            key[128 + kt] = log2f(v);
+            key[128 + kt] = log2f(v);                // (-inf for zeros)
             key[256 + kt] = v == v ? 1.f / v : 1.f;  // (NaN comes through the logarithm, to visible keys only)
+            if (v < 9.0949470e-13f || v > 1.0995116e12f) far[st] = g + 1;  // 2^-40, 2^40
           }
         }
         if (limit < 128) {  // the newest block's tokens, and zeros past them
@@ -478,6 +525,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
               const bool live = t + n < have, sane = h16_to_f(top[n], p.c.bf16) < INFINITY;
               const int e = live ? exponent_down(top[n], p.c.bf16) : 0;
               const float down = pow2f(-e);
+              const bool zero = live && top[n] == 0;
 #pragma unroll
               for (int x = 0; x < NV; ++x) {
                 const int piece = lane + 32 * x;
@@ -490,8 +538,9 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
                 }
               }
               if (lane == 0) {
-                key[128 + t + n] = sane ? static_cast<float>(e) : __uint_as_float(0x7fc00000u);
+                key[128 + t + n] = zero ? -INFINITY : sane ? static_cast<float>(e) : __uint_as_float(0x7fc00000u);
                 key[256 + t + n] = down;
+                if (zero || e < -40 || e > 40) far[st] = g + 1;
               }
             }
           }
@@ -521,23 +570,10 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
       // rows past the sequence's see nothing, and hide every key (a factor that is not positive needs the general form)
       const bool ragged = it.row0 + 128 * x + 128 > it.rows || !(p.scale_log2 > 0.f);
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < it.nkt; ++j) {
-        const int st = (g + j) % C::ST;
-        ok = mbar_wait_warp(&kv_full[st], (g + j) / C::ST & 1, abort_flag, DERR_WAIT_SLOT) &&
-             mbar_wait_warp(&s_full[x], (g + j) & 1, abort_flag, DERR_WAIT_MMA);
-        if (!ok) break;
-        tc_fence_after();
-        float s[128];
-        tmem_ld128(ts, s);
-        const float* key = reinterpret_cast<const float*>(smem + C::OFF_KEY) + st * 3 * C::BN;
-        const float qf = reinterpret_cast<const float*>(smem + C::OFF_QF)[(k & 1) * C::ROWS + 128 * x + rl];
-        float alpha;
-        if (ragged || 128 * j + 128 > min(least, it.full)) attn8_weights_each(s, key, qf, 128 * j, lim, m, l, alpha);
-        else attn8_weights(s, key, qf, m, l, alpha);
-        uint32_t pk[64];
-#pragma unroll
-        for (int c = 0; c < 64; ++c) pk[c] = pack_half2(s[2 * c], s[2 * c + 1]);
-        tmem_st64(ts, pk);
+      float* const ahead = reinterpret_cast<float*>(smem + C::OFF_AHEAD) + 128 * x + rl;
+      const float* const qfs = reinterpret_cast<const float*>(smem + C::OFF_QF) + (k & 1) * C::ROWS + 128 * x + rl;
+      // P is in place: O takes the new reference, and the MMA warp the weights
+      auto hand_over = [&](int j, float alpha) {
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -550,6 +586,40 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         }
         tc_fence_before();
         mbar_arrive(&p_full[x]);
+      };
+      int j = 0;
+      for (; j < it.nkt; ++j) {
+        const int st = (g + j) % C::ST;
+        ok = mbar_wait_warp(&kv_full[st], (g + j) / C::ST & 1, abort_flag, DERR_WAIT_SLOT);
+        if (!ok || __any_sync(0xffffffffu, far[st] == g + j + 1)) break;
+        ok = mbar_wait_warp(&s_full[x], (g + j) & 1, abort_flag, DERR_WAIT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        float s[128];
+        tmem_ld128(ts, s);
+        const float* key = reinterpret_cast<const float*>(smem + C::OFF_KEY) + st * 3 * C::BN;
+        const float qf = *qfs;
+        float alpha;
+        if (ragged || 128 * j + 128 > min(least, it.full)) attn8_weights_each(s, key, qf, 128 * j, lim, m, l, alpha);
+        else attn8_weights(s, key, qf, m, l, alpha);
+        uint32_t pk[64];
+#pragma unroll
+        for (int c = 0; c < 64; ++c) pk[c] = pack_half2(s[2 * c], s[2 * c + 1]);
+        tmem_st64(ts, pk);
+        hand_over(j, alpha);
+      }
+      const bool wide = ok && j < it.nkt;
+#pragma unroll 1
+      for (bool first = true; ok && j < it.nkt; ++j, first = false) {  // from the item's first far tile on
+        const int st = (g + j) % C::ST;
+        ok = mbar_wait_warp(&kv_full[st], (g + j) / C::ST & 1, abort_flag, DERR_WAIT_SLOT) &&
+             mbar_wait_warp(&s_full[x], (g + j) & 1, abort_flag, DERR_WAIT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        const float3 now = attn8_weights_far(ts, reinterpret_cast<const float*>(smem + C::OFF_KEY) + st * 3 * C::BN, *qfs,
+                                             128 * j, lim, m, l, ahead, first);
+        m = now.x, l = now.y;
+        hand_over(j, now.z);
       }
       if (!ok) break;
       if (it.nkt > 0) {
@@ -559,7 +629,8 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
         tc_fence_after();
       }
-      const float inv = lim > 0 ? 1.f / l : 0.f;  // a row that sees no key is 0
+      // a row that sees no key is 0; 2^-ahead in two halves, in fp32's range whatever the scales were
+      const float down = wide ? fast_exp2(-0.5f * *ahead) : 1.f, inv = lim > 0 ? 1.f / l * down : 0.f;
       const int tok = row / group;
       uint16_t* dst = p.out + (it.t0 + tok) * p.ld_out + static_cast<size_t>(it.head * group + row % group) * D;
 #pragma unroll 1
@@ -577,7 +648,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
             uint32_t w[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n)
-              w[n] = lim > 0 ? f_to_h16(o[e + 2 * n] * inv, p.c.bf16) | f_to_h16(o[e + 2 * n + 1] * inv, p.c.bf16) << 16 : 0u;
+              w[n] = lim > 0 ? f_to_h16(o[e + 2 * n] * inv * down, p.c.bf16) | f_to_h16(o[e + 2 * n + 1] * inv * down, p.c.bf16) << 16 : 0u;
             *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }

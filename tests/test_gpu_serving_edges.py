@@ -1,8 +1,12 @@
 """Corners of the 8-bit serving operators, on a B200: sequences shortened more than once, values and scales at the
 ends of their ranges, arguments that overlap or wrap, shapes that take the kernels' longer paths."""
 
+import math
+
 import pytest
 import torch
+
+from test_gpu_serving import U, Model, close, i32, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -10,14 +14,6 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(scope="module")
 def sv(tt):
     return tt.serving
-
-
-def i32(v):
-    return torch.tensor(v, dtype=torch.int32, device="cuda")
-
-
-def starts(counts):
-    return i32([0] + torch.tensor(counts).cumsum(0).tolist())
 
 
 # ------------------------------------------------------------------ shortened sequences
@@ -43,3 +39,73 @@ def test_decoder_rewound_twice(sv, tt):
         dec.forward(x[:38], [b], [38])
         y = dec.forward(torch.cat([x[38:41], x[38:41]]), [a, b], [3, 3])
         assert torch.equal(y[:3], y[3:])
+
+
+# ------------------------------------------------------------------ attention: values of very different sizes
+def compare(m, out, q, counts, heads, far):
+    """out against 64 bits.  A weight's relative error is test_gpu_serving's, and where V scales lie far from 1
+    (2^-125 .. 2^125: their logarithms are below 128, known to 2^-17, and enter two sums and a difference that round
+    alike) 4 * 2^-17 * ln 2 < 2^-15 more.  Weights carry V's scale and are held in fp16 times 2^14 of the largest:
+    2^-39 of the largest (weight times the largest value of a block) a key.  No absolute allowance but the type's
+    smallest step."""
+    g, at, d = heads // m.kv, 0, m.dim
+    for b, n in enumerate(counts):
+        length = m.lens[b]
+        k, v = m.seen(b, 0), m.seen(b, 1)
+        top = torch.zeros(length, m.kv, dtype=torch.float64, device="cuda")
+        for i in range(0, length, m.page):
+            top[i:i + m.page] = v[i:i + m.page].abs().amax((0, 2))
+        for i0 in range(0, n, 128):
+            i1 = min(n, i0 + 128)
+            x = q[at + i0:at + i1].double().view(i1 - i0, m.kv, g, d)
+            hide = torch.arange(length, device="cuda") > (length - n + torch.arange(i0, i1, device="cuda"))[:, None]
+            w = (torch.einsum("qhgd,khd->qhgk", x, k) / math.sqrt(d)).masked_fill(hide[:, None, None], -math.inf)
+            size = torch.einsum("qhgd,khd->qhgk", x.abs(), k.abs()).masked_fill(hide[:, None, None], 0).amax(-1, keepdim=True) / math.sqrt(d)
+            p = torch.softmax(w, -1)
+            ref = torch.einsum("qhgk,khd->qhgd", p, v).reshape(i1 - i0, heads, d)
+            eps = 2.0 ** -11 + 2.0 ** -20 + 2 * (d + 8) * 2.0 ** -24 * size + (2.0 ** -15 if far else 0)
+            err = torch.einsum("qhgk,khd->qhgd", 2 * eps * p, v.abs()).reshape(ref.shape)
+            low = length * 2.0 ** -39 * (p * top.T[None, :, None]).amax(-1).reshape(i1 - i0, heads, 1)
+            step = 2.0 ** -24 if m.dtype == torch.float16 else 2.0 ** -133
+            close(out[at + i0:at + i1], ref, err + low + U[m.dtype] * ref.abs() + step)
+        at += n
+
+
+@pytest.mark.parametrize("kv", [2, 16])  # the warps' kernel, and the 256-row kernel
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_many_values_of_zero_before_others(sv, pkg, dtype, kv):
+    """40000 keys of about equal weight whose values are zero, then 700 others: the sum of the weights must stay in
+    range, and the outputs are small averages."""
+    m = Model(sv, 1, kv, 64, 128, 41000, dtype)
+    k, v = kv * 64, 2 * kv * 64
+    x = m.rows(40700, 3 * kv * 64)
+    x[:, :v] *= 2 ** -4
+    x[:40000, v:] = 0
+    q = m.append([40700], kv, qkv=x)[40000:].contiguous()
+    out = m.c.attend(q, starts([700]), i32([40700]), max_q_len=700)
+    compare(m, out, q, [700], kv, False)
+    assert pkg.runtime.device_error() == 0
+
+
+@pytest.mark.parametrize("kv", [2, 16])
+def test_values_of_any_size(sv, kv):
+    """bf16 blocks of values from 2^-112 to 2^100, zeros between them and in the newest block: rows that see the small
+    ones only, and rows that see them beside large ones."""
+    sizes = [0, 2.0 ** -112, 2.0 ** -111, 0, 2.0 ** -60, 2.0 ** -38, 1.0, 0, 2.0 ** 50, 2.0 ** -30, 2.0 ** 100, 0]
+    m = Model(sv, 1, kv, 64, 64, 1024, torch.bfloat16)
+    v = 2 * kv * 64
+    x = m.rows(64 * len(sizes) + 50, 3 * kv * 64)
+    x[:, :v] *= 2 ** -3
+    for i, f in enumerate(sizes):
+        x[64 * i:64 * i + 64, v:] *= f
+    x[-50:-25, v:] = 0
+    x[-20:, v:] *= 2.0 ** 90
+    n = x.shape[0]
+    q = m.append([n], kv, qkv=x)
+    for upto in (n, n - 22, 64 * 6, 64 * 5 + 3):  # (shortened: what is read must not depend on what came later)
+        m.k[0], m.v[0] = m.k[0][:upto], m.v[0][:upto]
+        if upto < 64 * (len(sizes) - 1):
+            m = Model(sv, 1, kv, 64, 64, 1024, torch.bfloat16)
+            m.append([upto], kv, qkv=x[:upto])
+        out = m.c.attend(q[:upto].contiguous(), starts([upto]), i32([upto]), max_q_len=upto)
+        compare(m, out, q[:upto], [upto], kv, True)
