@@ -177,10 +177,9 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
          "qkv: the cache's 16-bit type, [tokens, (heads + 2 kv_heads) * D] expected");
     const int64_t tokens = qkv.size(0);
     int64_t ld = width;
-    if (tokens > 1) {
-      ld = qkv.stride(0);
-      need(qkv.stride(1) == 1 && ld % 8 == 0 && ld >= width, "qkv: dense rows that start 16-byte aligned and do not overlap expected");
-    }
+    if (tokens > 1) ld = qkv.stride(0);
+    need(tokens == 0 || (qkv.stride(1) == 1 && ld % 8 == 0 && ld >= width),
+         "qkv: dense rows that start 16-byte aligned and do not overlap expected");
     need(tokens <= 0x7fffffff, "sizes of 32 bits expected");
     int64_t rot = 0, turns = 0;
     if (cos || sin) {

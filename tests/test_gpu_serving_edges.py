@@ -109,3 +109,16 @@ def test_values_of_any_size(sv, kv):
             m.append([upto], kv, qkv=x[:upto])
         out = m.c.attend(q[:upto].contiguous(), starts([upto]), i32([upto]), max_q_len=upto)
         compare(m, out, q[:upto], [upto], kv, True)
+
+
+# ------------------------------------------------------------------ arguments
+def test_one_row_whose_channels_are_strided_is_refused(sv):
+    m = Model(sv, 1, 2, 64, 16, 64, torch.float16)
+    wide = m.rows(1, 2 * 6 * 64)
+    for strided in (wide[:, ::2], wide.view(6 * 64, 2).t()[:1]):
+        assert strided.shape == (1, 6 * 64) and strided.stride(1) == 2
+        with pytest.raises(ValueError):
+            m.c.append(strided, starts([1]), i32([0]), heads=2)
+    m.append([1], 2, qkv=wide[:, 8:8 + 6 * 64])  # a row of a wider buffer
+    assert m.c.append(wide[:0, ::2], starts([0]), i32([1]), heads=2).shape == (0, 2, 64)
+    m.check_read()
