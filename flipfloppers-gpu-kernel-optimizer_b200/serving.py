@@ -246,6 +246,8 @@ class Int8Decoder:
               f"x: contiguous fp32 [{total}, {cfg.d_model}] expected")
         _on_device(x)
         _need(all(self.lens[s] + c <= self.table.shape[1] * p for s, c in zip(seqs, counts)), "a sequence over max_tokens")
+        _need(all(c == 0 or self.lens[s] >= self.kept[s] for s, c in zip(seqs, counts)),
+              "a step of this sequence raised after it had overwritten what the sequence goes on from: close it")
         if total == 0:
             return torch.empty_like(x)
         new = [0] * n

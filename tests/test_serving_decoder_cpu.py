@@ -73,3 +73,34 @@ def test_a_sequence_that_was_closed_starts_afresh(decoder):
     decoder.step(s, 5)
     decoder.rewind(s, 5)
     decoder.step(s, 40)
+
+
+def test_a_step_that_failed(tt, decoder, monkeypatch):
+    """A step that raises half way has stored tokens already: it may be repeated where the slots still hold what
+    it starts from, and is refused where they do not."""
+    sv = tt.serving
+    good = sv.linear_int8
+    a, b = decoder.open(), decoder.open()
+    decoder.step(a, 20)
+    decoder.step(b, 20)
+
+    def broken(x, w, *args, resid=None, **kw):
+        if resid is not None:  # after the append and attention
+            raise RuntimeError("out of memory")
+        return good(x, w, *args, resid=resid, **kw)
+
+    for seq, n in ((a, 10), (b, 40)):
+        monkeypatch.setattr(sv, "linear_int8", broken)
+        with pytest.raises(RuntimeError):
+            decoder.step(seq, n)
+        monkeypatch.setattr(sv, "linear_int8", good)
+    assert decoder.lens[a] == decoder.lens[b] == 20
+    decoder.step(a, 10)
+    with pytest.raises(ValueError):
+        decoder.step(b, 40)  # the slot of block 1, whose first four tokens it needs, holds block 3
+    with pytest.raises(ValueError):
+        decoder.forward(torch.zeros(2, 64), [a, b], [1, 1])
+    decoder.step(a, 1)
+    decoder.close(b)
+    assert decoder.open() == b
+    decoder.step(b, 60)
