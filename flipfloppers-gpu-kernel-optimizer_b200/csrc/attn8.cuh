@@ -672,15 +672,21 @@ struct Attn8Warp {
   }
 };
 
-// sequence b's new tokens, clipped to what the buffers hold
-__device__ __forceinline__ void attn8_sequence(const Attn8Params& p, int b, int& t0, int& q_len, int& len) {
+// sequence b's new tokens; none where they or its length are outside the buffers.  false: cu decreases, so that
+// sequences could share rows and the line of work outgrow 32 bits: then nothing is computed at all.
+__device__ __forceinline__ bool attn8_sequence(const Attn8Params& p, int b, int& t0, int& q_len, int& len) {
   t0 = __ldg(p.cu + b);
-  q_len = __ldg(p.cu + b + 1) - t0;
+  const int end = __ldg(p.cu + b + 1);
   len = __ldg(p.lens + b);
-  if (t0 < 0 || q_len < 0 || t0 + q_len > p.tokens || len < 0 || len > static_cast<long long>(p.c.table_width) * p.c.page) {
+  q_len = 0;
+  if (t0 < 0 || end < t0 || end > p.tokens || len < 0 || len > static_cast<long long>(p.c.table_width) * p.c.page) {
     record_error(DERR_KV_RANGE);
-    t0 = q_len = len = 0;
+    const bool rises = end >= t0;
+    t0 = len = 0;
+    return rises;
   }
+  q_len = end - t0;
+  return true;
 }
 
 // OWN: a row tile a CTA, cut among its warps; else the line of units, cut among all warps.
@@ -696,13 +702,13 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
   fence_mbar_init();
   griddep_sync();
   const int group = p.heads / p.c.kv_heads;
-  int base = 0;
+  int base = 0, bad = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32 * C::WARPS) {
     const int b = b0 + tid;
     int n = 0;
     if (b < p.batch) {
       int t0, q_len, len;
-      attn8_sequence(p, b, t0, q_len, len);
+      bad |= !attn8_sequence(p, b, t0, q_len, len);
       n = p.c.kv_heads * ((q_len * group + C::ROWS - 1) / C::ROWS) * (OWN ? 1 : attn8_units(len, p.c.page));
     }
     int sum = n;
@@ -719,8 +725,9 @@ __global__ void __launch_bounds__(32 * Attn8Cfg<D, NT>::WARPS, 1) k_attn8(const 
       base += tot[i];
     }
     if (b < p.batch) line[b] = before + sum - n;
-    __syncthreads();
+    bad = __syncthreads_or(bad);
   }
+  if (bad) base = 0;
   if (tid == 0) line[p.batch] = base;
   __syncthreads();
   if (!OWN && blockIdx.x == 0)
@@ -868,8 +875,9 @@ __global__ void __launch_bounds__(ATTN8_JOIN_THREADS) k_attn8_join(const Attn8Pa
   attn8_sequence(p, b, t0, q_len, len);
   const int rt = u - (static_cast<int>(static_cast<long long>(__ldg(p.cu + b)) * group / C::ROWS) + b);
   const int tiles = (q_len * group + C::ROWS - 1) / C::ROWS;
-  if (rt < 0 || rt >= tiles) return;
-  const int units = attn8_units(len, p.c.page), total = p.plan[p.batch];
+  const int total = p.plan[p.batch];
+  if (rt < 0 || rt >= tiles || total == 0) return;
+  const int units = attn8_units(len, p.c.page);
   const int per = (total + p.warps - 1) / p.warps;
   const int first = p.plan[b] + (blockIdx.y * tiles + rt) * units;
   const int w0 = first / per, w1 = (first + units - 1) / per;

@@ -253,13 +253,13 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_sync();
-  int items = 0;
+  int items = 0, bad = 0;
   for (int b0 = 0; b0 < p.batch; b0 += C::THREADS) {
     const int b = b0 + tid;
     int n = 0;
     if (b < p.batch) {
       int t0, q_len, len;
-      attn8_sequence(p, b, t0, q_len, len);
+      bad |= !attn8_sequence(p, b, t0, q_len, len);
       n = p.c.kv_heads * ((q_len * group + 255) / 256);
     }
     int sum = n;
@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
       items += tot[i];
     }
     if (b < p.batch) line[b] = before + sum - n;
-    __syncthreads();
+    bad = __syncthreads_or(bad);
   }
+  if (bad) items = 0;
   const int G = gridDim.x;
 
   if (warp == 0) {

@@ -343,25 +343,31 @@ __global__ void __launch_bounds__(256, 4) k_kv8_append(const Kv8AppendParams p) 
   const int D = c.head_dim, P = c.page, psh = c.page_shift, u = blockIdx.x;
   const int k_ctas = (c.kv_heads + p.k_each - 1) / p.k_each;
   const int y = blockIdx.y, what = y < k_ctas ? 0 : y < 2 * k_ctas ? 1 : 2;
-  int b, blk;
+  int b;
+  if (p.by_token) b = warp_search(p.batch, u, [&](int i) { return __ldg(p.cu + i); });
+  // n tokens touch at most n/P + 2 blocks, so cu/P + 2b spaces the sequences apart
+  else b = warp_search(p.batch, u, [&](int i) { return (__ldg(p.cu + i) >> psh) + 2 * i; });
+  const int t0 = __ldg(p.cu + b), end = __ldg(p.cu + b + 1), start = __ldg(p.start + b);
+  if (t0 == end) return;
+  // (positions of whole blocks around the tokens fit 32 bits)
+  if (t0 < 0 || end < t0 || end > p.tokens || start < 0 || start > 0x7fffff00 - (end - t0)) {
+    if (tid == 0) record_error(DERR_KV_RANGE);
+    return;
+  }
+  const int n = end - t0, len = start + n;
+  int blk;
   if (p.by_token) {
-    b = warp_search(p.batch, u, [&](int i) { return __ldg(p.cu + i); });
-    const int t0 = __ldg(p.cu + b), pos = __ldg(p.start + b) + u - t0;
+    const int pos = start + u - t0;
     // the first token of a block in this call stands for the block
-    if (u < t0 || u >= __ldg(p.cu + b + 1) || (u != t0 && (pos & (P - 1)) != 0)) return;
+    if (u < t0 || u >= end || (u != t0 && (pos & (P - 1)) != 0)) return;
     blk = pos >> psh;
   } else {
-    // n tokens touch at most n/P + 2 blocks, so cu/P + 2b spaces the sequences apart
-    b = warp_search(p.batch, u, [&](int i) { return (__ldg(p.cu + i) >> psh) + 2 * i; });
-    blk = (__ldg(p.start + b) >> psh) + u - ((__ldg(p.cu + b) >> psh) + 2 * b);
+    blk = (start >> psh) + u - ((t0 >> psh) + 2 * b);
   }
-  const int t0 = __ldg(p.cu + b), start = __ldg(p.start + b);
-  const int n = __ldg(p.cu + b + 1) - t0, len = start + n;
   const int lo = max(start, blk * P), hi = min(len, (blk + 1) * P);  // positions of the block's new tokens
   if (lo >= hi) return;
   const int nrow = c.rows ? __ldg(c.rows + b) : b;
-  if (t0 < 0 || n < 0 || t0 + n > p.tokens || start < 0 || blk >= c.table_width || nrow < 0 || nrow >= c.new_rows ||
-      (p.cos && len > p.rope_rows)) {
+  if (blk >= c.table_width || nrow < 0 || nrow >= c.new_rows || (p.cos && len > p.rope_rows)) {
     if (tid == 0) record_error(DERR_KV_RANGE);
     return;
   }
@@ -429,9 +435,10 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Kv8ReadParams p) {
   const int pos = __ldg(p.start + b) + t - __ldg(p.cu + b), blk = pos >> c.page_shift, at = pos & (P - 1);
   const int nrow = c.rows ? __ldg(c.rows + b) : b;
   const size_t to = (static_cast<size_t>(t) * c.kv_heads + head) * D + d;
-  const bool full = (blk + 1) * P <= __ldg(p.lens + b);
+  const bool full = blk < __ldg(p.lens + b) >> c.page_shift;
   const int page = blk < c.table_width && pos >= 0 ? __ldg(c.table + static_cast<size_t>(b) * c.table_width + blk) : -1;
-  if (pos < 0 || (full ? page < 0 || page >= c.num_pages : nrow < 0 || nrow >= c.new_rows)) {
+  // (rows past the last sequence's are nobody's: their positions may be anything)
+  if (pos < 0 || (blk >= c.table_width && t < __ldg(p.cu + b + 1)) || (full ? page < 0 || page >= c.num_pages : nrow < 0 || nrow >= c.new_rows)) {
     record_error(DERR_KV_RANGE);
     *reinterpret_cast<uint4*>(p.k_out + to) = make_uint4(0, 0, 0, 0);
     *reinterpret_cast<uint4*>(p.v_out + to) = make_uint4(0, 0, 0, 0);

@@ -328,7 +328,7 @@ int b200_block_forward_noalloc(const B200BlockArgs* args, b200_stream_t stream);
  * table [batch][table_width]: the page of each block of each sequence.
  * head_dim 32, 64 or 128; page_size 16, 32, 64 or 128; batch <= 2048.  All on the
  * device, 16-byte aligned.  A page, row or length outside its buffer is skipped
- * and sets the device error word (7). */
+ * and sets the device error word (7); where cu decreases, attention computes nothing. */
 typedef struct {
   void* k_pages;
   void* v_pages;

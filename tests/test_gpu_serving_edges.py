@@ -122,3 +122,42 @@ def test_one_row_whose_channels_are_strided_is_refused(sv):
     m.append([1], 2, qkv=wide[:, 8:8 + 6 * 64])  # a row of a wider buffer
     assert m.c.append(wide[:0, ::2], starts([0]), i32([1]), heads=2).shape == (0, 2, 64)
     m.check_read()
+
+
+@pytest.mark.parametrize("cu", [[2 ** 31 - 1, -2, 3], [0, 8, 0], [-2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1], [0, -1, 8], [0, 2 ** 31 - 1, -2 ** 31]])
+@pytest.mark.parametrize("wide", [128, 9000, 100000])
+def test_rows_that_wrap_or_decrease_are_reported_not_followed(sv, pkg, cu, wide):
+    """cu whose differences leave 32 bits, or that decreases: no rows, the error word, and the cache as it was (but for the
+    sequences whose own rows are in order, which append takes one by one)."""
+    m = Model(sv, 2, 2, 64, 16, wide, torch.float16)
+    m.append([40, 20], 2)
+    before = [t.clone() for t in m.c.tensors[:6]]
+    for n, most in ((8, 4), (8000, 4000)):
+        heads = 2
+        q = m.rows(n, heads * 64).view(n, heads, 64)
+        out = torch.full_like(q, 7.0)
+        assert pkg.runtime.device_error() == 0
+        m.c.attend(q, i32(cu), i32([40, 20]), max_q_len=most, out=out)
+        assert pkg.runtime.device_error() == 7 and bool((out == 7).all())
+        m.c.append(m.rows(n, 6 * 64), i32(cu), i32([40, 20]), heads=2)
+        assert pkg.runtime.device_error() == 7
+        if cu == [0, 8, 0]:  # the first sequence's rows are as they should be: append stores them
+            continue
+        for t, was in zip(m.c.tensors[:6], before):
+            assert torch.equal(t.view(torch.uint8), was.view(torch.uint8))
+
+
+def test_starts_that_wrap_are_reported_not_followed(sv, pkg):
+    m = Model(sv, 2, 2, 64, 16, 128, torch.float16)
+    m.append([40, 20], 2)
+    before = [t.clone() for t in m.c.tensors[:6]]
+    for n in (1, 10, 300):
+        for start in (2 ** 31 - 1, 2 ** 31 - 5, -1, -2 ** 31):
+            m.c.append(m.rows(n, 6 * 64), starts([n, 0]), i32([start, 2 ** 31 - 1]), heads=2)
+            assert pkg.runtime.device_error() == 7
+            m.c.read(starts([n, 0]), i32([start, 0]), i32([40, 20]), total=n)
+            assert pkg.runtime.device_error() == 7
+    m.c.append(m.rows(3, 6 * 64), starts([0, 3]), i32([-1, 20]), heads=2)  # no new tokens: its start is not looked at
+    assert pkg.runtime.device_error() == 0
+    for t, was in zip(m.c.tensors[:4], before):
+        assert torch.equal(t.view(torch.uint8), was.view(torch.uint8))
