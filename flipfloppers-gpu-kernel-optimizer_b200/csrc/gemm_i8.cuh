@@ -46,8 +46,8 @@ __device__ __forceinline__ void load_row16(const void* x, size_t base, int k, in
 // 2048 rows or more of up to 2048 values (32768x1024 fp16 in 23 us, 4.4 TB/s), else 256
 // (333x1001 bf16: the product 10.2 us, with a warp a row 12.7); the row is read twice,
 // the second time from L1.
-// Memory-bound.  vec: x's rows start 16-byte aligned; ldq is a multiple of 16 or the
-// codes leave one by one.
+// Memory-bound.  vec: x's rows start 16-byte aligned.  Only the K codes of a row are
+// written, 16 at a time where they start on 16 bytes.
 template <int DT, int TPR>
 __global__ void __launch_bounds__(256) k_quant_rows(const void* x, long long ldx, int8_t* q, long long ldq,
                                                     float* scale, int M, int K, int vec) {
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) k_quant_rows(const void* x, long long ldx
       w.w = quantize4(v[12], v[13], v[14], v[15], s, inv, small);
     }
     int8_t* to = q + row * ldq + k;
-    if (k + 16 <= ldq && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+    if (k + 16 <= K && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
       *reinterpret_cast<uint4*>(to) = w;
     } else {
       const uint32_t x[4] = {w.x, w.y, w.z, w.w};

@@ -161,3 +161,19 @@ def test_starts_that_wrap_are_reported_not_followed(sv, pkg):
     assert pkg.runtime.device_error() == 0
     for t, was in zip(m.c.tensors[:4], before):
         assert torch.equal(t.view(torch.uint8), was.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float16, 0), (torch.bfloat16, 1), (torch.float32, 2)])
+@pytest.mark.parametrize("m,k", [(3, 1), (5, 17), (2, 100), (2100, 40), (2100, 1009), (7, 5000)])
+def test_quantized_rows_leave_their_neighbours_alone(pkg, dtype, code, m, k):
+    """Codes as a range of columns of a wider buffer: nothing beside them is written."""
+    x = torch.randn(m, (k + 23) // 8 * 8, device="cuda").to(dtype)
+    wide = torch.full((m, k + 48 - k % 16), 99, dtype=torch.int8, device="cuda")
+    scale = torch.empty(m, device="cuda")
+    rc = pkg.runtime.lib().b200_quantize_rows_i8(x.data_ptr(), code, x.shape[1], wide.data_ptr() + 16, wide.shape[1],
+                                                 scale.data_ptr(), m, k, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    top = x[:, :k].float().abs().amax(1)
+    assert torch.equal(scale, top * (1 / 127))
+    assert torch.equal(wide[:, 16:16 + k].float(), (x[:, :k].float() / scale[:, None]).round())
+    assert bool((wide[:, :16] == 99).all()) and bool((wide[:, 16 + k:] == 99).all())
