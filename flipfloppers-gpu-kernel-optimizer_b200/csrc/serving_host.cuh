@@ -335,8 +335,8 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   if (!a->x || !a->w || !a->w_scale || !a->out) return B200_ERR_ARG;
   if (a->ld_x < a->k || a->ld_w < a->k || a->ld_out < a->n || (a->resid && a->ld_resid < a->n)) return B200_ERR_ARG;
   if (a->ld_w % 16 || !al16(a->w)) return B200_ERR_ALIGN;
-  // the sums are int32: |sum| <= 127 * 127 * k
-  if (a->k > 133000) return B200_ERR_TILE;
+  // the sums are int32: |sum| <= 127 * 128 * k (a weight may use the code -128)
+  if (a->k > 0x7fffffff / (127 * 128)) return B200_ERR_TILE;
   const bool few = lin_small_fits(a->m, a->k);
   if (!few) {
     if (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k)) return B200_ERR_WORKSPACE;
