@@ -38,7 +38,7 @@ constexpr int ATTN8_MAX_BATCH = 2048;
 
 struct Attn8Params {
   Kv8Cache c;
-  const uint16_t* q;     // [tokens, heads, D], row stride ld_q
+  const uint16_t* q;     // [tokens, heads, D], row stride ld_q; may be `out`, so it is not read with __ldg
   uint16_t* out;         // [tokens, heads, D], row stride ld_out
   long long ld_q, ld_out;
   const int* cu;         // [batch + 1] first row of each sequence's new tokens
@@ -478,7 +478,7 @@ struct Attn8Warp {
         if constexpr (BF16) {  // rows in their own type: read again
           bool live;
           const uint16_t* from = row_ptr(s.rt * C::ROWS + 8 * n + g, live) + chan(j);
-          uint2 q0 = __ldg(reinterpret_cast<const uint2*>(from)), q1 = __ldg(reinterpret_cast<const uint2*>(from + 4));
+          uint2 q0 = *reinterpret_cast<const uint2*>(from), q1 = *reinterpret_cast<const uint2*>(from + 4);
           if (!live) q0 = q1 = make_uint2(0, 0);
           mma_bf16(sc[0][n], a0, q0.x, q0.y);
           mma_bf16(sc[0][n], a1, q1.x, q1.y);

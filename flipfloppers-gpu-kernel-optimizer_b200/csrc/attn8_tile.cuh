@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         if (p.c.bf16 && live) {
           unsigned top = 0;
           for (int d = 0; d < D; d += 8) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + d));
+            const uint4 w = *reinterpret_cast<const uint4*>(src + d);
             top = top2(top2(top2(top2(top, w.x), w.y), w.z), w.w);
           }
           const int e = exponent_down(max(top & 0xffffu, top >> 16), 1);
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
           down = pow2f(-e);
         }
         for (int d = 0; d < D; d += 8) {
-          uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(src + d)) : make_uint4(0, 0, 0, 0);
+          uint4 w = live ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
           if (p.c.bf16) w = scale8(w, 1, down);
           *reinterpret_cast<uint4*>(smem + (r >> 7) * C::Q_BYTES + attn8_off<D>(128, r & 127, d)) = w;
         }

@@ -190,12 +190,12 @@ __device__ __forceinline__ void i8_epilogue(const CUtensorMap* tmO, const GemmI8
         if (p.vec_resid && col + CC <= p.N) {
 #pragma unroll
           for (int j = 0; j < CC; j += 4) {
-            const float4 w = __ldg(reinterpret_cast<const float4*>(r + j));
+            const float4 w = *reinterpret_cast<const float4*>(r + j);  // (not __ldg: resid may be out)
             u[j] = w.x; u[j + 1] = w.y; u[j + 2] = w.z; u[j + 3] = w.w;
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < CC; ++j) u[j] = col + j < p.N ? __ldg(r + j) : 0.f;
+          for (int j = 0; j < CC; ++j) u[j] = col + j < p.N ? r[j] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < CC; ++j)
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(32 * LIN_MAX_WARPS, 1) k_lin_small(const __gri
       for (int c = 0; c < LIN_MAX_CLUSTER; ++c) sum += each[c];
       float y = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(sum), sx[m]), sw), bias);
       if (p.epi == I8_GELU) y = gelu_as(y);
-      if (p.epi == I8_RESID) y = __fadd_rn(__ldg(p.g.resid + m * p.g.ld_resid + col), y);
+      if (p.epi == I8_RESID) y = __fadd_rn(p.g.resid[m * p.g.ld_resid + col], y);
       const long long to = m * p.g.ld_out + col;
       if (p.out_type == DT_F32) static_cast<float*>(p.g.out)[to] = y;
       else static_cast<uint16_t*>(p.g.out)[to] = static_cast<uint16_t>(f_to_h16(y, p.out_type == DT_BF16));
