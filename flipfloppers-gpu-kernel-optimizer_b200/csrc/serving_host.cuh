@@ -7,6 +7,23 @@
 
 namespace {
 
+// `rows` rows of `width` bytes, `pitch` bytes apart
+struct Rows8 {
+  const void* at;
+  long long rows, pitch, width;
+};
+// Whether two such ranges share a byte (columns of one wider buffer may lie side by side).
+bool overlap(const Rows8& a, const Rows8& b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0) return false;
+  const auto a0 = reinterpret_cast<uintptr_t>(a.at), b0 = reinterpret_cast<uintptr_t>(b.at);
+  if (a0 + (a.rows - 1) * a.pitch + a.width <= b0 || b0 + (b.rows - 1) * b.pitch + b.width <= a0) return false;
+  const long long pitch = a.rows > 1 ? a.pitch : b.pitch;
+  if ((a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) || pitch <= 0) return true;
+  long long d = static_cast<long long>(b0 - a0) % pitch;  // b's first column in a's rows
+  if (d < 0) d += pitch;
+  return d < a.width || d + b.width > pitch;
+}
+
 int cache8_check(const B200KvCache8* c) {
   if (!c || !c->k_pages || !c->v_pages || !c->k_scale || !c->v_scale || !c->k_newest || !c->v_newest || !c->table)
     return B200_ERR_ARG;
@@ -53,6 +70,8 @@ int kv8_append_impl(const B200KvCache8* c, const void* qkv, long long ld, void* 
   if (cos && (rot <= 0 || rot % 16 || rot > c->head_dim || rope_rows <= 0)) return B200_ERR_TILE;
   if (ld < static_cast<long long>(heads + 2 * c->kv_heads) * c->head_dim) return B200_ERR_ARG;
   if (!al16(qkv) || !al16(q_out) || !al16(cos) || !al16(sin) || ld % 8) return B200_ERR_ALIGN;
+  const long long row = static_cast<long long>(heads) * c->head_dim * 2;
+  if (overlap({q_out, tokens, row, row}, {qkv, tokens, ld * 2, row + 4LL * c->kv_heads * c->head_dim})) return B200_ERR_ARG;
   if (int rc = check_arch()) return rc;
   Kv8AppendParams p{};
   p.c = cache8_of(c);
@@ -199,6 +218,9 @@ int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, 
   const long long chunks = static_cast<long long>(c->table_width) * c->page_size / ATTN8_CHUNK + 1 + ATTN8_START + 8 * ATTN8_NEWEST;
   if (rows > 0x7fffffffLL || (rows / 8 + c->batch) * c->kv_heads * chunks > 0x7fffffffLL) return B200_ERR_TILE;
   if (!ws || ws_bytes < attn8_workspace(c->batch, heads, c->kv_heads, c->head_dim, max_q_len)) return B200_ERR_WORKSPACE;
+  // a row tile is written after it was read, so `out` may be q itself
+  if ((out != q || (tokens > 1 && ld_out != ld_q)) && overlap({out, tokens, ld_out * 2, width * 2}, {q, tokens, ld_q * 2, width * 2}))
+    return B200_ERR_ARG;
   if (!al16(ws)) return B200_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   Attn8Params p{};
@@ -338,10 +360,16 @@ int linear_i8_impl(const B200LinearI8Args* a, cudaStream_t st) {
   // the sums are int32: |sum| <= 127 * 128 * k (a weight may use the code -128)
   if (a->k > 0x7fffffff / (127 * 128)) return B200_ERR_TILE;
   const bool few = lin_small_fits(a->m, a->k);
-  if (!few) {
-    if (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k)) return B200_ERR_WORKSPACE;
-    if (!al16(a->workspace)) return B200_ERR_ALIGN;
-  }
+  if (!few && (!a->workspace || a->workspace_bytes < linear_i8_workspace(a->m, a->k))) return B200_ERR_WORKSPACE;
+  // the epilogue reads an element of resid before it writes it, so `out` may be resid itself; x and w are read throughout
+  const long long esize = a->out_type == DT_F32 ? 4 : 2, xsize = a->x_type == DT_F32 ? 4 : 2;
+  const Rows8 out{a->out, a->m, a->ld_out * esize, a->n * esize};
+  if (overlap(out, {a->x, a->m, a->ld_x * xsize, a->k * xsize}) || overlap(out, {a->w, a->n, a->ld_w, a->k}) ||
+      overlap(out, {a->w_scale, 1, 0, 4LL * a->n}) || overlap(out, {a->bias, 1, 0, 4LL * a->n}))
+    return B200_ERR_ARG;
+  if ((a->resid != a->out || (a->m > 1 && a->ld_resid != a->ld_out)) && overlap(out, {a->resid, a->m, a->ld_resid * 4, 4LL * a->n}))
+    return B200_ERR_ARG;
+  if (!few && !al16(a->workspace)) return B200_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   GemmI8Params p{};
   p.M = a->m;

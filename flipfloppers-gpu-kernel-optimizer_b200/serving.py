@@ -127,7 +127,8 @@ class PagedKV8:
         ``qkv`` [tokens, (heads + 2 kv_heads) * D] (q, k, v heads side by side; the rows may be
         strided): row cu[b] + i is token start[b] + i of sequence b (``cu`` int32 [batch + 1],
         ``start`` int32 [batch]).  ``cos`` / ``sin`` fp32 [positions, rot / 2]: the first ``rot``
-        channels of a head turn in pairs (i, i + rot/2), or (2i, 2i + 1) if ``interleaved``."""
+        channels of a head turn in pairs (i, i + rot/2), or (2i, 2i + 1) if ``interleaved``.  ``out``
+        may not overlap qkv."""
         return _done(_module.append(self._c, qkv, cu, start, heads, cos, sin, interleaved, out), "b200_kv8_append")
 
     def read(self, cu: Tensor, start: Tensor, lens: Tensor, *, total: int) -> Tuple[Tensor, Tensor]:
@@ -141,7 +142,8 @@ class PagedKV8:
 
         Row cu[b] + i of ``q`` is the token at position lens[b] - n + i of sequence b (n = cu[b+1] -
         cu[b] <= ``max_q_len``), appended already; it sees the keys up to its own.  A row with no key
-        gives zeros.  ``scale`` defaults to 1 / sqrt(D).  The same inputs give the same bits."""
+        gives zeros.  ``scale`` defaults to 1 / sqrt(D).  ``out`` may be q itself, and not overlap it
+        otherwise.  The same inputs give the same bits."""
         return _done(_module.attend(self._c, q, cu, lens, max_q_len, scale, out), "b200_kv8_attention")
 
 
@@ -167,7 +169,7 @@ def linear_int8(x: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = 
     ``x`` [m, k] fp16, bf16 or fp32 (rows may be strided); ``w`` int8 [n, pitch], pitch a multiple
     of 16, at least k (``quantize_weight``); ``w_scale`` and ``bias`` fp32 [n].  With ``gelu`` the
     exact GELU follows.  ``resid`` fp32 [m, n] is added last: the result is fp32, and ``out`` may be
-    ``resid`` itself.  Without it the result has ``out_dtype`` (default: x's type)."""
+    ``resid`` itself; it may not overlap what is read otherwise.  Without it the result has ``out_dtype`` (default: x's type)."""
     return _done(_native().linear_i8(x, w, w_scale, bias, gelu, resid, out_dtype, out), "b200_linear_i8")
 
 

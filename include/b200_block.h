@@ -347,7 +347,8 @@ typedef struct {
  * rotated by position (the first `rot` channels of a head, a multiple of 16; pairs
  * (i, i + rot/2), or (2i, 2i+1) if interleaved; cos and sin fp32
  * [rope_rows, rot/2]; cos NULL: no rotation), q goes to q_out
- * [tokens, heads, head_dim], k and v to the cache.  cu [batch+1], start [batch]. */
+ * [tokens, heads, head_dim], k and v to the cache.  cu [batch+1], start [batch].  q_out
+ * may not overlap qkv. */
 int b200_kv8_append(const B200KvCache8* cache, const void* qkv, long long ld_qkv, void* q_out, const int* cu,
                     const int* start, const float* cos, const float* sin, int rot, int interleaved, int rope_rows,
                     int tokens, int heads, b200_stream_t stream);
@@ -364,7 +365,7 @@ int b200_kv8_read(const B200KvCache8* cache, const int* cu, const int* start, co
  * to its own; heads % kv_heads == 0, consecutive query heads share a key head.  A
  * row with no key (position < 0) gives zeros.  What is not finite in the newest block
  * reaches the rows that see it and no others (NaN, or the infinity in its channel).
- * max_q_len >= every n.  No atomics:
+ * max_q_len >= every n.  out may be q itself, and not overlap it otherwise.  No atomics:
  * the same inputs give the same bits. */
 size_t b200_kv8_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int max_q_len);
 int b200_kv8_attention(const B200KvCache8* cache, const void* q, long long ld_q, void* out, long long ld_out,
@@ -375,7 +376,7 @@ int b200_kv8_attention(const B200KvCache8* cache, const void* q, long long ld_q,
  * sx = the row's largest magnitude / 127 and exact integer sums.  x [m, k] of x_type,
  * w int8 [n, k] with row pitch ld_w (a multiple of 16 bytes), bias fp32 or NULL, gelu
  * != 0: exact GELU; resid (fp32 [m, n], out_type fp32, no GELU) is added last and may
- * be out itself.  Types: 0 fp16, 1 bf16, 2 fp32.  Any m, n, k up to k = 132104.  A row
+ * be out itself; out may not overlap what is read otherwise.  Types: 0 fp16, 1 bf16, 2 fp32.  Any m, n, k up to k = 132104.  A row
  * with an infinity or NaN gives NaN. */
 typedef struct {
   const void* x;

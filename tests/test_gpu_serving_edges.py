@@ -177,3 +177,33 @@ def test_quantized_rows_leave_their_neighbours_alone(pkg, dtype, code, m, k):
     assert torch.equal(scale, top * (1 / 127))
     assert torch.equal(wide[:, 16:16 + k].float(), (x[:, :k].float() / scale[:, None]).round())
     assert bool((wide[:, :16] == 99).all()) and bool((wide[:, 16 + k:] == 99).all())
+
+
+def test_outputs_over_inputs(sv, pkg):
+    """out may be q (attention) and resid (linear); what overlaps otherwise is refused, columns side by side are not."""
+    refused = pkg.runtime.B200Error
+    for kv, n, most in ((2, 3, 128), (2, 3, 9000), (16, 800, 1024)):  # the warps' two ways, the 256-row kernel
+        for dtype in (torch.float16, torch.bfloat16):
+            m = Model(sv, 1, kv, 64, 16, most, dtype)
+            q = m.append([n + 90], 2 * kv)[90:].contiguous()
+            want = m.c.attend(q, starts([n]), i32(m.lens), max_q_len=n)
+            assert m.c.attend(q, starts([n]), i32(m.lens), max_q_len=n, out=q) is q and torch.equal(q, want)
+            both = torch.zeros(n, 4 * kv * 64, dtype=dtype, device="cuda")
+            left, right = (both[:, i:i + 2 * kv * 64].view(n, 2 * kv, 64) for i in (0, 2 * kv * 64))
+            m.c.attend(left, starts([n]), i32(m.lens), max_q_len=n, out=right)
+            with pytest.raises(refused):
+                m.c.attend(q[1:], starts([n - 1]), i32(m.lens), max_q_len=n, out=q[:-1])
+    qkv = m.rows(2, 6 * 16 * 64)
+    with pytest.raises(refused):
+        m.c.append(qkv[:1], starts([1]), i32(m.lens), heads=64, out=qkv[:1, :64 * 64].view(1, 64, 64))
+    w, ws = sv.quantize_weight(torch.randn(64, 64, device="cuda"))
+    for rows in (5, 100):
+        x = torch.randn(rows, 128, device="cuda")
+        y = x.clone()
+        want = sv.linear_int8(x[:, :64], w, ws)
+        sv.linear_int8(x[:, :64], w, ws, out=x[:, 64:])
+        assert torch.equal(x[:, 64:], want) and torch.equal(x[:, :64], y[:, :64])
+        with pytest.raises(refused):
+            sv.linear_int8(x[:, :64], w, ws, out=x[:, :64])
+        with pytest.raises(refused):
+            sv.linear_int8(y[:, :64], w, ws, resid=x[:, :64], out=x[:, 4:68])
