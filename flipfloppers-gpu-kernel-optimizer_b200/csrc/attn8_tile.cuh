@@ -16,8 +16,8 @@
 // From the first such tile of an item on, the sum takes exponentials of the scores themselves, twice as many, with a
 // reference of its own, and V of zeros weighs nothing in the products.  The newest block's
 // 16-bit values are brought into fp16 by a power of two for each token (exact to 2^-24
-// of the token's largest value); a token whose V has an infinity or NaN gives NaN to the
-// rows that see it and nothing to the others.
+// of the token's largest value); infinities and NaN of its V stay out of the products (0 times them would reach rows
+// that do not see the token) and join their channel of the rows that see them at the end.
 // Bound: the softmax (the exponentials alone, 16 a clock and SM, take 2048 clocks for two 128x128 tiles; a row's 128
 // weights take its one thread about 2500).  Measured: 2048 tokens over 17200 keys, 16 heads of 64, 343 us (397 TFLOP/s);
 // 1024 tokens over 8000 keys, 32/8 heads of 128, 255 us.
@@ -98,6 +98,79 @@ __device__ __forceinline__ uint4 scale8(uint4 w, int bf16, float f) {  // eight 
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 __device__ __forceinline__ unsigned top2(unsigned top, uint32_t w) { return __vmaxu2(top, w & 0x7fff7fffu); }
+
+// The newest block's 16-bit tokens as keys [first, have) of a tile, zeros past them, by the three converting warps.  Once
+// an item, and a call of its own, so that the codes' registers are not spilled for it (1024 tokens over 8000 keys of 32/8
+// heads of 128: 263 us inlined, 257 so).
+template <int D>
+__device__ __noinline__ void attn8_newest(const uint16_t* k_new, const uint16_t* v_new, int bf16, int first, int have,
+                                          uint8_t* ks, uint8_t* vs, float* key, int* far, int tile, int* odd, int item) {
+  const int lane = threadIdx.x & 31, cw = (threadIdx.x >> 5) - 1;
+  constexpr int LK = D / 8, TK = 32 / LK;  // lanes a token, tokens a warp
+  for (int t0 = first + cw * TK; t0 < 128; t0 += 3 * TK) {
+    const int t = t0 + lane / LK, d = lane % LK * 8;
+    const bool live = t < have;
+    uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(k_new + (t - first) * D + d)) : make_uint4(0, 0, 0, 0);
+    unsigned top = top2(top2(top2(top2(0u, w.x), w.y), w.z), w.w);
+    top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+    for (int x = 1; x < LK; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const int e = exponent_down(top, bf16);
+    if (t < 128) {
+      *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, t, d)) = scale8(w, bf16, pow2f(-e));
+      if (d == 0) key[t] = pow2f(e);
+    }
+  }
+  for (int t = first + 4 * cw; t < 128; t += 12) {  // four tokens a warp
+    constexpr int NV = D == 128 ? 2 : 1;             // 16-byte pieces (two channels of four tokens) a lane
+    uint4 w[NV];
+    const unsigned most = bf16 ? 0x7f7fu : 0x7bffu;  // the largest finite magnitude
+    unsigned top[4] = {0, 0, 0, 0};
+    unsigned strange = 0;  // bit n: token t + n has a value that is not finite
+#pragma unroll
+    for (int x = 0; x < NV; ++x) {
+      const int piece = lane + 32 * x;
+      w[x] = piece < D / 2 && t < have
+                 ? __ldg(reinterpret_cast<const uint4*>(v_new + (t - first) * D + piece * 8)) : make_uint4(0, 0, 0, 0);
+      const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const unsigned a = u[n >> 1] >> (16 * (n & 1)) & 0x7fffu, b = u[2 + (n >> 1)] >> (16 * (n & 1)) & 0x7fffu;
+        top[n] = max(top[n], max(a <= most ? a : 0u, b <= most ? b : 0u));
+        if (t + n < have && max(a, b) > most) strange |= 1u << n;
+      }
+    }
+    strange = __reduce_or_sync(0xffffffffu, strange);
+    if (strange && lane == 0) *odd = item;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      top[n] = __reduce_max_sync(0xffffffffu, top[n]);
+      const bool live = t + n < have;
+      // (a token with nothing else than zeros, infinities and NaN: small, and no far one)
+      const int e = !live ? 0 : top[n] == 0 && (strange >> n & 1) ? -40 : exponent_down(top[n], bf16);
+      const float down = pow2f(-e);
+      const bool zero = live && top[n] == 0 && !(strange >> n & 1);
+#pragma unroll
+      for (int x = 0; x < NV; ++x) {
+        const int piece = lane + 32 * x;
+        const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+        if (piece < D / 2) {
+          float a = h16_to_f(u[n >> 1] >> (16 * (n & 1)) & 0xffffu, bf16);
+          float b = h16_to_f(u[2 + (n >> 1)] >> (16 * (n & 1)) & 0xffffu, bf16);
+          if (!(fabsf(a) < INFINITY)) a = 0.f;
+          if (!(fabsf(b) < INFINITY)) b = 0.f;
+          *reinterpret_cast<uint32_t*>(vs + attn8_off<D>(128, t + n, 2 * piece)) =
+              live ? pack_half2(a * down, b * down) : 0u;
+        }
+      }
+      if (lane == 0) {
+        key[128 + t + n] = zero ? -INFINITY : static_cast<float>(e);
+        key[256 + t + n] = down;
+        if (zero || e < -40 || e > 40) *far = tile;
+      }
+    }
+  }
+}
 
 // One softmax step of a row: raw scores s (in registers) become weights.  Key factors in shared memory: K scale,
 // log2 of the V scale, 1 / V scale.
@@ -208,6 +281,21 @@ __device__ __forceinline__ float3 attn8_weights_far(uint32_t ts, const float* ke
   return make_float3(now, (l * fast_exp2(lwas - base) + sum) * fast_exp2(fminf(0.f, over)), fast_exp2(m - top));
 }
 
+// Infinities and NaN among the first n tokens of the newest block's V take their channel of a finished row.  Rare, and
+// a call of its own, which leaves the registers of the rest alone.
+__device__ __noinline__ void attn8_strange(const uint16_t* v, int n, int dim, int bf16, uint16_t* out) {
+#pragma unroll 1
+  for (int d = 0; d < dim; ++d) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int t = 0; t < n; ++t) {
+      const float a = h16_to_f(__ldg(v + ((t >> 2) * dim + d) * 4 + (t & 3)), bf16);
+      if (!(fabsf(a) < INFINITY)) sum += a;
+    }
+    if (sum != 0.f) out[d] = static_cast<uint16_t>(f_to_h16(sum + h16_to_f(out[d], bf16), bf16));  // (what is NaN already stays)
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(const Attn8Params p) {
   using C = Attn8TileCfg<D>;
@@ -226,6 +314,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* far = reinterpret_cast<int*>(tmem_slot + 2);  // [ST] of the stage's tile: its number plus 1 if it is a far one
+  int* odd = far + C::ST;  // [4] of the item: its number plus 1 if the newest V is not all finite
   int* line = reinterpret_cast<int*>(smem + C::TOTAL);  // [batch + 1] first item of each sequence
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.heads / p.c.kv_heads;
@@ -240,7 +329,7 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
       mbar_init(&o_done[i], 1);
     }
     mbar_init(drain, 1);
-    *abort_flag = far[0] = far[1] = 0;
+    *abort_flag = far[0] = far[1] = odd[0] = odd[1] = odd[2] = odd[3] = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -489,62 +578,8 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
           if (!good && i == 0) record_error(DERR_KV_RANGE);
           const size_t base = ((static_cast<size_t>(good ? nrow : 0) * 2 + (it.full >> psh & 1)) * p.c.kv_heads + it.head) *
                               static_cast<size_t>(P * D);
-          constexpr int LK = D / 8, TK = 32 / LK;  // lanes a token, tokens a warp
-          for (int t0 = first + cw * TK; t0 < 128; t0 += 3 * TK) {
-            const int t = t0 + lane / LK, d = lane % LK * 8;
-            const bool live = good && t < have;
-            uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(p.c.k_new + base + (t - first) * D + d)) : make_uint4(0, 0, 0, 0);
-            unsigned top = top2(top2(top2(top2(0u, w.x), w.y), w.z), w.w);
-            top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-            for (int x = 1; x < LK; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const int e = exponent_down(top, p.c.bf16);
-            if (t < 128) {
-              *reinterpret_cast<uint4*>(ks + attn8_off<D>(128, t, d)) = scale8(w, p.c.bf16, pow2f(-e));
-              if (d == 0) key[t] = pow2f(e);
-            }
-          }
-          for (int t = first + 4 * cw; t < 128; t += 12) {  // four tokens a warp
-            constexpr int NV = D == 128 ? 2 : 1;             // 16-byte pieces (two channels of four tokens) a lane
-            uint4 w[NV];
-            unsigned top[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int x = 0; x < NV; ++x) {
-              const int piece = lane + 32 * x;
-              w[x] = good && piece < D / 2 && t < have
-                         ? __ldg(reinterpret_cast<const uint4*>(p.c.v_new + base + (t - first) * D + piece * 8)) : make_uint4(0, 0, 0, 0);
-              const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
-#pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                const unsigned a = u[n >> 1] >> (16 * (n & 1)) & 0x7fffu, b = u[2 + (n >> 1)] >> (16 * (n & 1)) & 0x7fffu;
-                top[n] = max(top[n], max(a, b));
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              top[n] = __reduce_max_sync(0xffffffffu, top[n]);
-              const bool live = t + n < have, sane = h16_to_f(top[n], p.c.bf16) < INFINITY;
-              const int e = live ? exponent_down(top[n], p.c.bf16) : 0;
-              const float down = pow2f(-e);
-              const bool zero = live && top[n] == 0;
-#pragma unroll
-              for (int x = 0; x < NV; ++x) {
-                const int piece = lane + 32 * x;
-                const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
-                if (piece < D / 2) {
-                  const float a = h16_to_f(u[n >> 1] >> (16 * (n & 1)) & 0xffffu, p.c.bf16);
-                  const float b = h16_to_f(u[2 + (n >> 1)] >> (16 * (n & 1)) & 0xffffu, p.c.bf16);
-                  *reinterpret_cast<uint32_t*>(vs + attn8_off<D>(128, t + n, 2 * piece)) =
-                      live && sane ? pack_half2(a * down, b * down) : 0u;
-                }
-              }
-              if (lane == 0) {
-                key[128 + t + n] = zero ? -INFINITY : sane ? static_cast<float>(e) : __uint_as_float(0x7fc00000u);
-                key[256 + t + n] = down;
-                if (zero || e < -40 || e > 40) far[st] = g + 1;
-              }
-            }
-          }
+          attn8_newest<D>(p.c.k_new + base, p.c.v_new + base, p.c.bf16, first, good ? have : 0, ks, vs, key, far + st, g + 1,
+                          odd + (k & 3), k + 1);
         }
         fence_proxy_async_smem();
         mbar_arrive(&kv_full[st]);
@@ -623,6 +658,8 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
         hand_over(j, now.z);
       }
       if (!ok) break;
+      // (the word is another item's three on at the earliest: this warp has then handed over a tile of the next)
+      const bool strange = it.nkt > 0 && odd[k & 3] == k + 1;
       if (it.nkt > 0) {
         g += it.nkt;
         ++k;
@@ -653,6 +690,11 @@ __global__ void __launch_bounds__(Attn8TileCfg<D>::THREADS, 1) k_attn8_tile(cons
             *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+      }
+      if (strange && row < it.rows) {
+        const int nrow = p.c.rows ? __ldg(p.c.rows + it.b) : it.b;  // (in range: the token was read from there)
+        attn8_strange(p.c.v_new + ((static_cast<size_t>(nrow) * 2 + (it.full / p.c.page & 1)) * p.c.kv_heads + it.head) *
+                                      static_cast<size_t>(p.c.page * D), lim - it.full, D, p.c.bf16, dst);
       }
       tc_fence_before();
     }

@@ -207,3 +207,36 @@ def test_outputs_over_inputs(sv, pkg):
             sv.linear_int8(x[:, :64], w, ws, out=x[:, :64])
         with pytest.raises(refused):
             sv.linear_int8(y[:, :64], w, ws, resid=x[:, :64], out=x[:, 4:68])
+
+
+# ------------------------------------------------------------------ infinities and NaN
+@pytest.mark.parametrize("kv", [2, 16])  # the warps' kernel, and the 256-row kernel
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("page", [16, 128])
+def test_values_that_are_not_finite_stay_in_their_channel(sv, dtype, kv, page):
+    """Infinities and NaN among the newest block's values: their channel of the rows that see them, nothing else."""
+    n = 7 * 128 + 13
+    m = Model(sv, 2, kv, 64, page, 1024, dtype)
+    v = 2 * kv * 64
+    x = m.rows(2 * n, 3 * kv * 64)
+    x[:, :v] *= 2 ** -3   # (flat weights: none is 0, whose product with an infinity is NaN)
+    clean = x.clone()
+    x[n - 11, v + 7] = math.inf              # head 0
+    x[n - 9, v + 9] = -math.inf
+    x[n - 4, v + 7] = -math.inf              # inf and -inf: NaN
+    x[n - 10, v + 64:v + 128] = math.nan     # head 1: all of a token's channels
+    x[2 * n - 1, v + 5] = math.nan           # the other sequence's last token
+    q = m.c.append(x, starts([n, n]), i32([0, 0]), heads=kv)
+    out = m.c.attend(q, starts([n, n]), i32([n, n]), max_q_len=n)
+    m.append([n, n], kv, qkv=clean, start=[0, 0])
+    want = m.check_attend(q, [n, n], kv)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    assert bool((out[n - 11:n - 4, 0, 7] == math.inf).all()) and bool(out[n - 4:n, 0, 7].isnan().all())
+    assert bool((out[n - 9:n, 0, 9] == -math.inf).all())
+    assert bool(out[n - 10:n, 1].isnan().all()) and bool(out[2 * n - 1, 0, 5].isnan())
+    bad[n - 11:n, 0, 7] = bad[n - 9:n, 0, 9] = bad[n - 10:n, 1] = bad[2 * n - 1, 0, 5] = True
+    assert bool(out[~bad].isfinite().all())
+    # elsewhere what the rows give without them, within the two calls' own errors (a token's power of two may differ):
+    # 2^-10 of the average of |v|, which is below 6, and the rounding
+    off = (out.double() - want.double()).abs()[~bad]
+    assert bool((off <= 2 * (2.0 ** -10 * 6 + U[dtype] * want.double().abs()[~bad])).all())
