@@ -167,8 +167,8 @@ def linear_int8(x: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = 
     """epi((round(x / sx) @ w.T) * sx * w_scale + bias), sx = each row's largest magnitude / 127.
 
     ``x`` [m, k] fp16, bf16 or fp32 (rows may be strided); ``w`` int8 [n, pitch], pitch a multiple
-    of 16, at least k (``quantize_weight``); ``w_scale`` and ``bias`` fp32 [n].  With ``gelu`` the
-    exact GELU follows.  ``resid`` fp32 [m, n] is added last: the result is fp32, and ``out`` may be
+    of 16, at least k (``quantize_weight``); ``w_scale`` and ``bias`` fp32 [n].  With ``gelu``
+    the erf form of GELU follows (fp32 results: to fp32; 16-bit ones: within 2e-6).  ``resid`` fp32 [m, n] is added last: the result is fp32, and ``out`` may be
     ``resid`` itself; it may not overlap what is read otherwise.  Without it the result has ``out_dtype`` (default: x's type)."""
     return _done(_native().linear_i8(x, w, w_scale, bias, gelu, resid, out_dtype, out), "b200_linear_i8")
 

@@ -375,7 +375,7 @@ int b200_kv8_attention(const B200KvCache8* cache, const void* q, long long ld_q,
 /* out[M,N] = epi( (round(x / sx) . w^T) * sx[row] * w_scale[col] + bias[col] ) with
  * sx = the row's largest magnitude / 127 and exact integer sums.  x [m, k] of x_type,
  * w int8 [n, k] with row pitch ld_w (a multiple of 16 bytes), bias fp32 or NULL, gelu
- * != 0: exact GELU; resid (fp32 [m, n], out_type fp32, no GELU) is added last and may
+ * != 0: GELU by erf (fp32 results to fp32, 16-bit ones within 2e-6); resid (fp32 [m, n], out_type fp32, no GELU) is added last and may
  * be out itself; out may not overlap what is read otherwise.  Types: 0 fp16, 1 bf16, 2 fp32.  Any m, n, k up to k = 132104.  A row
  * with an infinity or NaN gives NaN. */
 typedef struct {

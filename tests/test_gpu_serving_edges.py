@@ -240,3 +240,28 @@ def test_values_that_are_not_finite_stay_in_their_channel(sv, dtype, kv, page):
     # 2^-10 of the average of |v|, which is below 6, and the rounding
     off = (out.double() - want.double()).abs()[~bad]
     assert bool((off <= 2 * (2.0 ** -10 * 6 + U[dtype] * want.double().abs()[~bad])).all())
+
+
+# ------------------------------------------------------------------ int8 linear
+def linear64(sv, m, k, n, dtype, seed, spread=3.0):
+    """x, a quantized weight, and (round(x / sx) w) sx sw in 64 bits."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = (torch.randn(m, k, generator=g, device="cuda") * spread).to(dtype)
+    w, ws = sv.quantize_weight(torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k))
+    xs = x.float().abs().amax(1, keepdim=True) * (1 / 127)
+    xc = (x.float() / xs).round().clamp(-127, 127)
+    return x, w, ws, (xc.double() @ w[:, :k].double().T) * xs.double() * ws.double()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,k,n", [(1, 256, 512), (64, 512, 200), (100, 300, 130), (600, 256, 512), (520, 1152, 300)])
+def test_gelu_of_fp32_results_is_exact_to_fp32(sv, m, k, n, dtype):
+    """y is off by six fp32 roundings; erff by 2 ulp (2^-23 near 1), its argument by 2^-23 (which moves erf by less than
+    that), 1 + erf by 2^-24 of at most 2, and two products by 2^-24 each: |y| / 2 * 3 * 2^-23 and 2^-23 of the result."""
+    x, w, ws, part = linear64(sv, m, k, n, dtype, m + k)
+    bias = torch.randn(n, device="cuda")
+    y = sv.linear_int8(x, w, ws, bias, gelu=True, out_dtype=torch.float32)
+    size = part.abs() + bias.abs().double()
+    part = part + bias.double()
+    ref = torch.nn.functional.gelu(part)
+    close(y, ref, 1.13 * 6 * 2.0 ** -24 * size + 1.5 * 2.0 ** -23 * part.abs() + 2.0 ** -23 * ref.abs() + 2.0 ** -60)
