@@ -158,7 +158,7 @@ int launch_attn8(Attn8Params& p, long long rows, cudaStream_t st) {
   // no second kernel.  Measured (line against CTA, us on the device, one token a sequence): 1 x 1000 keys of 16 heads of
   // 64: 12.1, 8.4; 8 x 2000: 18.0, 11.2; 16 x 1000 (288 tiles): 19.5, 15.5; 16 x 1000 keys of 32/8 heads of 128: 19.1,
   // 11.1; past the bounds 1 x 4000: 13.2, 16.5; 32 x 1000 (576 tiles): 26.2, 28.9; 4 x 3000 of 32/8 heads: 17.3, 20.0.
-  const long long tiles = (rows / C::ROWS + p.batch) * p.c.kv_heads;
+  const long long tiles = (rows / C::ROWS + std::min(p.batch, p.tokens)) * p.c.kv_heads;
   const bool own = tiles <= 2 * ctas && static_cast<long long>(p.c.table_width) * p.c.page / ATTN8_CHUNK <= 4 * C::WARPS;
   static_assert(C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4 + 128 <= 227 * 1024, "ring and line fit an SM");
   auto kern = own ? k_attn8<D, NT, SMALL, true> : k_attn8<D, NT, SMALL, false>;
@@ -179,7 +179,7 @@ int launch_attn8_tile(Attn8Params& p, long long rows, cudaStream_t st) {
   constexpr int most = C::TOTAL + (ATTN8_MAX_BATCH + 1) * 4 + 1024;
   static_assert(most <= 227 * 1024, "tiles and line fit an SM");
   if (int rc = set_smem(reinterpret_cast<const void*>(kern), most)) return rc;
-  const long long items = (rows / 256 + p.batch) * p.c.kv_heads;
+  const long long items = (rows / 256 + std::min(p.batch, p.tokens)) * p.c.kv_heads;
   launch_kernel(kern, dim3(static_cast<unsigned>(std::min<long long>(items, num_sms()))), dim3(C::THREADS),
                 C::TOTAL + (p.batch + 1) * 4 + 1024, st, p);
   return launch_status();
@@ -189,15 +189,19 @@ int launch_attn8_tile(Attn8Params& p, long long rows, cudaStream_t st) {
 // over the SMs, theirs by the rows (new tokens times query heads); a wave takes as long as this many rows.  Measured
 // (warps against tiles, us): 8192 rows over 8000 keys, D = 128: 222, 212; D = 64: 147, 165; D = 32: 117, 145;
 // 16384 rows, D = 128: 425, 215; D = 64: 274, 166; 8 x 256 rows of 16 heads over 2000 keys, D = 32: 122, 49; 4096
-// rows of D = 128: 123, 213.
-bool attn8_many_rows(long long rows, int kv_heads, int batch, int head_dim) {
-  const long long items = (rows / batch + 255) / 256 * batch * kv_heads, waves = (items + num_sms() - 1) / num_sms();
+// rows of D = 128: 123, 213.  The items are counted as if the sequences with new tokens had max_q_len each: sequences
+// without any, the idle slots of a batch, count for nothing (1 token of 1 of 16 sequences, 8000 keys of 16 heads of 64:
+// 14, 245).  One choice for the batch: single tokens beside a chunk that fills the tiles go with it.
+bool attn8_many_rows(int tokens, int max_q_len, int group, int kv_heads, int head_dim) {
+  const long long rows = static_cast<long long>(tokens) * group, each = std::min<long long>(static_cast<long long>(max_q_len) * group, rows);
+  const long long busy = (static_cast<long long>(tokens) + max_q_len - 1) / max_q_len;
+  const long long items = (each + 255) / 256 * busy * kv_heads, waves = (items + num_sms() - 1) / num_sms();
   return rows * kv_heads >= waves * (head_dim == 128 ? 8000 : 10000);
 }
 
 template <int D>
-int launch_attn8_d(Attn8Params& p, bool one, long long rows, cudaStream_t st) {
-  if (attn8_many_rows(rows, p.c.kv_heads, p.batch, D)) return launch_attn8_tile<D>(p, rows, st);
+int launch_attn8_d(Attn8Params& p, bool one, bool many, long long rows, cudaStream_t st) {
+  if (many) return launch_attn8_tile<D>(p, rows, st);
   if (p.c.page == 16) return one ? launch_attn8<D, 1, true>(p, rows, st) : launch_attn8<D, 2, true>(p, rows, st);
   return one ? launch_attn8<D, 1, false>(p, rows, st) : launch_attn8<D, 2, false>(p, rows, st);
 }
@@ -236,11 +240,11 @@ int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, 
   p.heads = heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = static_cast<float*>(ws);
-  const bool one = attn8_rows(max_q_len, group) == 8;
+  const bool one = attn8_rows(max_q_len, group) == 8, many = attn8_many_rows(tokens, max_q_len, group, c->kv_heads, c->head_dim);
   switch (c->head_dim) {
-    case 32: return launch_attn8_d<32>(p, one, rows, st);
-    case 64: return launch_attn8_d<64>(p, one, rows, st);
-    default: return launch_attn8_d<128>(p, one, rows, st);
+    case 32: return launch_attn8_d<32>(p, one, many, rows, st);
+    case 64: return launch_attn8_d<64>(p, one, many, rows, st);
+    default: return launch_attn8_d<128>(p, one, many, rows, st);
   }
 }
 

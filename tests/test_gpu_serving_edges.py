@@ -265,3 +265,23 @@ def test_gelu_of_fp32_results_is_exact_to_fp32(sv, m, k, n, dtype):
     part = part + bias.double()
     ref = torch.nn.functional.gelu(part)
     close(y, ref, 1.13 * 6 * 2.0 ** -24 * size + 1.5 * 2.0 ** -23 * part.abs() + 2.0 ** -23 * ref.abs() + 2.0 ** -60)
+
+
+# ------------------------------------------------------------------ attention: which kernel
+@pytest.mark.parametrize("kv,group,new", [(16, 1, 1), (4, 3, 2), (8, 4, 30)])
+def test_idle_slots_change_nothing(sv, kv, group, new):
+    """A sequence among 31 that have no new tokens is attended to as it is alone: by the warps' kernel, whose work is
+    cut alike then, so the bits are the same."""
+    n = 3000
+    alone = Model(sv, 1, kv, 64, 64, 9000, torch.float16, seed=1)
+    among = Model(sv, 32, kv, 64, 64, 9000, torch.float16, seed=2)
+    heads = kv * group
+    x = alone.rows(n, (heads + 2 * kv) * 64)
+    q = alone.append([n], heads, qkv=x)[n - new:].contiguous()
+    counts = [0] * 32
+    counts[17] = n
+    among.append(counts, heads, qkv=x)
+    counts[17] = new
+    want = alone.check_attend(q, [new], heads)
+    got = among.c.attend(q, starts(counts), i32(among.lens), max_q_len=new)
+    assert torch.equal(got, want)
