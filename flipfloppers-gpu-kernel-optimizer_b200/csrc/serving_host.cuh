@@ -218,9 +218,12 @@ int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, 
   if (!al16(q) || !al16(out) || ld_q % 8 || ld_out % 8) return B200_ERR_ALIGN;
   const int group = heads / c->kv_heads;
   const long long rows = static_cast<long long>(tokens) * group;
-  // the line of (sequence, head, row tile, unit) work is numbered in 32 bits
+  // rows, and items of 256 rows and a key head, are numbered in 32 bits, and the warps' line of (sequence, head, row tile,
+  // unit) work: what is too long for that goes to the 256-row kernel
+  if (rows > 0x7fffffffLL || (rows / 256 + c->batch) * c->kv_heads > 0x7fffffffLL) return B200_ERR_TILE;
   const long long chunks = static_cast<long long>(c->table_width) * c->page_size / ATTN8_CHUNK + 1 + ATTN8_START + 8 * ATTN8_NEWEST;
-  if (rows > 0x7fffffffLL || (rows / 8 + c->batch) * c->kv_heads * chunks > 0x7fffffffLL) return B200_ERR_TILE;
+  const bool many = (rows / 8 + c->batch) * c->kv_heads > 0x7fffffffLL / chunks ||
+                    attn8_many_rows(tokens, max_q_len, group, c->kv_heads, c->head_dim);
   if (!ws || ws_bytes < attn8_workspace(c->batch, heads, c->kv_heads, c->head_dim, max_q_len)) return B200_ERR_WORKSPACE;
   // a row tile is written after it was read, so `out` may be q itself
   if ((out != q || (tokens > 1 && ld_out != ld_q)) && overlap({out, tokens, ld_out * 2, width * 2}, {q, tokens, ld_q * 2, width * 2}))
@@ -240,7 +243,7 @@ int attn8_impl(const B200KvCache8* c, const void* q, long long ld_q, void* out, 
   p.heads = heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = static_cast<float*>(ws);
-  const bool one = attn8_rows(max_q_len, group) == 8, many = attn8_many_rows(tokens, max_q_len, group, c->kv_heads, c->head_dim);
+  const bool one = attn8_rows(max_q_len, group) == 8;
   switch (c->head_dim) {
     case 32: return launch_attn8_d<32>(p, one, many, rows, st);
     case 64: return launch_attn8_d<64>(p, one, many, rows, st);

@@ -285,3 +285,15 @@ def test_idle_slots_change_nothing(sv, kv, group, new):
     want = alone.check_attend(q, [new], heads)
     got = among.c.attend(q, starts(counts), i32(among.lens), max_q_len=new)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 0, 2], [40, 1, 300, 7]])
+def test_attend_in_a_table_of_a_billion_positions(sv, pkg, new):
+    m = Model(sv, 4, 16, 64, 64, 1024, torch.float16)
+    m.append([700, 0, 64, 130], 16)
+    q = m.append(new, 16)
+    table = torch.zeros(4, 1 << 24, dtype=torch.int32, device="cuda")
+    table[:, :m.table.shape[1]] = m.table
+    m.c = sv.PagedKV8(*m.c.tensors[:6], table)
+    m.check_attend(q, new, 16)
+    assert pkg.runtime.device_error() == 0

@@ -89,3 +89,19 @@ def test_append_refuses_outputs_that_overlap(pkg):
 
     for out, tokens in ((qkv, 3), (qkv, 1), (qkv + 512, 1), (qkv + 1008, 1), (qkv - 496, 1), (qkv + 3 * 1024 - 16, 3), (qkv - 1024, 3)):
         assert append(out, tokens) == -9, (out - qkv, tokens)
+
+
+def test_attention_over_wide_tables_is_taken(pkg):
+    """Work that the warps' kernel could not number in 32 bits goes to the other one, which has no such line."""
+    rt = pkg.runtime
+
+    def attend(c, tokens, most, heads):  # -5: a workspace off 16 bytes, looked at last
+        return rt.lib().b200_kv8_attention(c, 1 << 20, 64 * heads, 1 << 40, 64 * heads, 256, 64, tokens, heads, most, 1.0, 4097,
+                                           1 << 40, None)
+
+    wide = kv8(rt, kv_heads=16, table_width=1 << 24)
+    assert attend(wide, 1, 1, 16) == -5
+    assert attend(wide, 4, 1, 16) == -5
+    assert attend(kv8(rt, kv_heads=8, table_width=4096, batch=2048), 1 << 19, 256, 64) == -5
+    assert attend(kv8(rt, kv_heads=1024), 0x7fffffff, 1 << 20, 1024) == -2   # items of 256 rows that 32 bits do not number
+    assert attend(kv8(rt), 0x7fffffff, 1 << 20, 4) == -2                     # rows that 32 bits do not number
