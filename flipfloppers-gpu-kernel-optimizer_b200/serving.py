@@ -12,8 +12,9 @@
 
 Everything runs on the current stream of the tensors' device, never synchronises
 and raises on arguments the kernels do not take; there is no other implementation
-behind it.  Row counts and lengths are device tensors (int32), so that a step can
-be captured in a CUDA graph and replayed with other values in them.
+behind it.  The operators' row counts and lengths are device tensors (int32), so
+that a step written with them can be captured in a CUDA graph and replayed with
+other values in them (``Int8Decoder`` counts on the host, and is not captured).
 """
 
 from __future__ import annotations
@@ -253,22 +254,31 @@ class Int8Decoder:
         if total == 0:
             return torch.empty_like(x)
         new = [0] * n
+        grown, pages = [], []  # sequences that need pages and how many; the pages
         for s, c in zip(seqs, counts):
             new[s] = c
-            self.kept[s] = max(self.kept[s], ((self.lens[s] + c - 1) // p - 1) * p)
-            grown = []
-            while len(self.pages[s]) * p < self.lens[s] + c:
-                self.pages[s].append(self.spare.pop())
-                grown.append(self.pages[s][-1])
-            if grown:
-                first = len(self.pages[s]) - len(grown)
-                self.table[s, first:first + len(grown)] = torch.tensor(grown, dtype=torch.int32).to(self.dev)
+            more = (self.lens[s] + c + p - 1) // p - len(self.pages[s])
+            if more > 0:
+                grown.append((s, more))
+                end = len(self.spare) - len(pages)
+                pages += self.spare[end - more:end][::-1]
         start = [max(0, length) for length in self.lens]
         cu = [0]
         for c in new:
             cu.append(cu[-1] + c)
-        meta = torch.tensor(cu + start + [a + b for a, b in zip(start, new)], dtype=torch.int32).to(self.dev)
-        cu_t, start_t, lens_t = meta[:n + 1], meta[n + 1:2 * n + 1], meta[2 * n + 1:]
+        # one copy from pinned memory, which the allocator keeps until the copy has run: nothing waits for the device
+        meta = torch.tensor(cu + start + [a + b for a, b in zip(start, new)] + pages, dtype=torch.int32,
+                            pin_memory=self.dev.type == "cuda").to(self.dev, non_blocking=True)
+        cu_t, start_t, lens_t, pages_t = meta.split([n + 1, n, n, len(pages)])
+        at = 0
+        for s, more in grown:
+            had = len(self.pages[s])
+            self.table[s, had:had + more] = pages_t[at:at + more]
+            self.pages[s] += pages[at:at + more]
+            del self.spare[-more:]
+            at += more
+        for s, c in zip(seqs, counts):
+            self.kept[s] = max(self.kept[s], ((self.lens[s] + c - 1) // p - 1) * p)
         res = x.clone()
         norm = torch.empty(x.shape, dtype=torch.float16, device=self.dev)
         for w in self.layers:

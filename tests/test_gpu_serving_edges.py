@@ -297,3 +297,39 @@ def test_attend_in_a_table_of_a_billion_positions(sv, pkg, new):
     m.c = sv.PagedKV8(*m.c.tensors[:6], table)
     m.check_attend(q, new, 16)
     assert pkg.runtime.device_error() == 0
+
+
+# ------------------------------------------------------------------ the decoder and the host
+def test_decoder_steps_do_not_wait_for_the_device(sv, tt):
+    """No call of a step synchronises, new pages or not, and steps that are issued far ahead of the device give what
+    steps one by one give (the host's buffers are not used again too early)."""
+    cfg = tt.TransformerConfig(1, 64, 256, 4, 512, 2, True)
+    torch.manual_seed(6)
+    model = tt.UserOptimizedTransformer(cfg).cuda().eval()
+    prompt = torch.randn(40, 256, device="cuda")
+    outs = []
+    with torch.inference_mode():
+        for ahead in (False, True):
+            dec = sv.Int8Decoder(model, max_sequences=3, max_tokens=160, page_size=16)
+            a, b = dec.open(), dec.open()
+            y = dec.forward(prompt, [a, b], [25, 15])
+            dec.forward(y[:1].contiguous(), [a], [1])
+            dec.rewind(a, 1)
+            x = torch.stack([y[24], y[39]])
+            got = []
+            torch.cuda.synchronize()
+            if ahead:
+                torch.cuda._sleep(200_000_000)  # (0.1 s: the steps below are all issued meanwhile)
+            torch.cuda.set_sync_debug_mode("error")
+            try:
+                for i in range(100):
+                    x = dec.forward(x, [a, b], [1, 1])
+                    got.append(x)
+                    if not ahead:
+                        torch.cuda.set_sync_debug_mode("default")
+                        torch.cuda.synchronize()
+                        torch.cuda.set_sync_debug_mode("error")
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+            outs.append(torch.stack(got))
+    assert torch.equal(*outs)
