@@ -224,15 +224,18 @@ class Int8Decoder:
         self.lens[seq] = self.kept[seq] = 0
         return seq
 
+    def _open_length(self, seq: int) -> int:
+        _need(0 <= seq < len(self.lens) and self.lens[seq] >= 0, f"sequence {seq} is not open")
+        return self.lens[seq]
+
     def close(self, seq: int) -> None:
-        _need(self.lens[seq] >= 0, f"sequence {seq} is not open")
+        self._open_length(seq)
         self.spare += reversed(self.pages[seq])
         self.pages[seq], self.lens[seq] = [], -1
 
     def rewind(self, seq: int, n: int) -> None:
         """Drop the last n tokens of a sequence."""
-        length = self.lens[seq]
-        _need(length >= 0, f"sequence {seq} is not open")
+        length = self._open_length(seq)
         _need(0 <= n <= length and (n == 0 or length - n >= self.kept[seq]),
               "rewind reaches back to the first token of the newest two blocks the sequence has had")
         self.lens[seq] = length - n

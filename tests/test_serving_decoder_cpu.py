@@ -104,3 +104,17 @@ def test_a_step_that_failed(tt, decoder, monkeypatch):
     decoder.close(b)
     assert decoder.open() == b
     decoder.step(b, 60)
+
+
+def test_ids_that_are_no_sequence_are_refused(decoder):
+    ids = [decoder.open() for _ in range(3)]
+    for s in ids:
+        decoder.step(s, 5)
+    for bad in (-1, -3, 3, 100):
+        for call in (lambda: decoder.rewind(bad, 1), lambda: decoder.close(bad), lambda: decoder.step(bad, 1)):
+            with pytest.raises(ValueError):
+                call()
+    assert decoder.lens == [5, 5, 5]
+    decoder.close(2)
+    with pytest.raises(ValueError):
+        decoder.close(2)
