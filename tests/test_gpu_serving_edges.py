@@ -333,3 +333,32 @@ def test_decoder_steps_do_not_wait_for_the_device(sv, tt):
                 torch.cuda.set_sync_debug_mode("default")
             outs.append(torch.stack(got))
     assert torch.equal(*outs)
+
+
+# ------------------------------------------------------------------ int8 linear: every lap of the rings
+@pytest.mark.parametrize("epi", ["bias", "gelu", "resid"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,k,n", [
+    (2500, 700, 2100),    # CTA pairs: 90 tiles on 74 pairs, two laps of K's ring; 16 epilogue warps for GELU
+    (5000, 1160, 2061),   # 180 tiles, a third for some pairs; 8 epilogue warps; rows of out off 16 bytes
+    (700, 2300, 300),     # few tiles of a long K
+    (511, 700, 10000),    # 128x128 tiles: 316 on 148 CTAs, a third for some
+    (3000, 650, 250),     # 128x128 tiles of few columns
+])
+def test_linear_of_many_tiles(sv, pkg, m, k, n, dtype, epi):
+    x, w, ws, part = linear64(sv, m, k, n, dtype, m + n)
+    bias = torch.randn(n, device="cuda")
+    resid = torch.randn(m, n, device="cuda") if epi == "resid" else None
+    y = sv.linear_int8(x, w, ws, bias, gelu=epi == "gelu", resid=resid)
+    bound = 6 * 2.0 ** -24 * (part.abs() + bias.abs().double())  # test_gpu_serving's bounds
+    part = part + bias.double()
+    if epi == "gelu":
+        part = torch.nn.functional.gelu(part)
+        bound = 1.2 * bound + 2.0 ** -18 * (1 + part.abs())
+    if epi == "resid":
+        part = part + resid.double()
+        bound = bound + 2.0 ** -24 * part.abs()
+    close(y, part, bound + 2.0 ** -40 + U[y.dtype] * part.abs() + (2.0 ** -25 if y.dtype != torch.float32 else 0))
+    if epi == "resid":  # in place: the same bits
+        assert torch.equal(sv.linear_int8(x, w, ws, bias, resid=resid, out=resid), y)
+    assert pkg.runtime.device_error() == 0
