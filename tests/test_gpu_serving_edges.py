@@ -362,3 +362,63 @@ def test_linear_of_many_tiles(sv, pkg, m, k, n, dtype, epi):
     if epi == "resid":  # in place: the same bits
         assert torch.equal(sv.linear_int8(x, w, ws, bias, resid=resid, out=resid), y)
     assert pkg.runtime.device_error() == 0
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 9000, 130), (64, 8193, 64), (3, 20000, 17), (64, 8192, 200)])
+def test_linear_of_few_rows_and_a_long_k(sv, m, k, n):
+    """Few rows whose K the cluster's shared memory does not hold, and one that it just does."""
+    x, w, ws, part = linear64(sv, m, k, n, torch.bfloat16, k)
+    y = sv.linear_int8(x, w, ws, out_dtype=torch.float32)
+    close(y, part, 6 * 2.0 ** -24 * part.abs() + 2.0 ** -40)
+
+
+def test_linear_beyond_31_bits(sv):
+    """An output whose offsets pass 2^31 elements, rows of x and of the residual that start beyond 2^31."""
+    x, w, ws, part = linear64(sv, 300, 64, 20000, torch.float16, 1)
+    big = x.repeat(400, 1)[:110000]
+    y = sv.linear_int8(big, w, ws)
+    assert y.numel() > 2 ** 31
+    for at in (0, 107700, 109800 - 300):
+        part_at = part.roll(-(at % 300), 0)[:300]
+        close(y[at:at + 300], part_at, 6 * 2.0 ** -24 * part_at.abs() + U[torch.float16] * part_at.abs() + 2.0 ** -25)
+    del y
+    wide = torch.zeros(80, 2 ** 26, dtype=torch.float16, device="cuda")
+    wide[:, -64:] = x[:80]
+    for rows in (40, 80):
+        y = sv.linear_int8(wide[:rows, -64:], w, ws)
+        close(y, part[:rows], 6 * 2.0 ** -24 * part[:rows].abs() + U[torch.float16] * part[:rows].abs() + 2.0 ** -25)
+
+
+# ------------------------------------------------------------------ the cache at its limits
+def test_rows_beyond_31_bits(sv, pkg):
+    """qkv, queries and outputs whose rows lie 2^26 elements apart."""
+    m = Model(sv, 2, 2, 64, 16, 64, torch.float16)
+    wide = torch.zeros(40, 2 ** 26, dtype=torch.float16, device="cuda")
+    wide[:, 72:72 + 8 * 64] = m.rows(40, 8 * 64)
+    q = m.append([22, 18], 4, qkv=wide[:, 72:72 + 8 * 64])
+    m.check_read()
+    wide[:, 1024:1024 + 256] = q.view(40, 256)
+    far, out = (wide[:, i:i + 256].view(40, 4, 64) for i in (1024, 2048))
+    m.c.attend(far, starts([22, 18]), i32(m.lens), max_q_len=22, out=out)
+    m.compare(out, q, [22, 18], 4)
+    assert pkg.runtime.device_error() == 0
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_the_largest_batch(sv, pkg, new):
+    m = Model(sv, 2048, 1, 32, 16, 48, torch.bfloat16)
+    m.append([(i * 7) % 30 for i in range(2048)], 2)
+    counts = [new if i % 5 else 0 for i in range(2048)]
+    q = m.append(counts, 2)
+    m.check_read()
+    m.check_attend(q, counts, 2)
+    assert pkg.runtime.device_error() == 0
+
+
+@pytest.mark.parametrize("group,new,before", [(71, 1, 500), (40, 3, 77), (64, 300, 10), (128, 1, 3000)])
+def test_many_query_heads_share_a_key_head(sv, pkg, group, new, before):
+    m = Model(sv, 2, 1, 64, 32, 4096, torch.float16)
+    m.append([before, 5], group)
+    q = m.append([new, 1], group)
+    m.check_attend(q, [new, 1], group)
+    assert pkg.runtime.device_error() == 0
