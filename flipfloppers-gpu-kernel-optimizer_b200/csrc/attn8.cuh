@@ -32,7 +32,10 @@
 namespace b200 {
 
 constexpr int ATTN8_CHUNK = 32;   // tokens
-// Weights are kept times 2^14 (at most 16384), so that fp16 has eleven bits for those down to 2^-28 of the largest.
+// Weights meet V in fp16 (in the newest block of a bf16 cache as two bf16 parts), scores, maxima and sums are fp32: a
+// weight is off by at most 2^-11 of itself, so an output by less than one rounding of an fp16 result, where weights of
+// more bits would take a second product (twice the tensor steps of PV).  They are kept times 2^14 (at most 16384), so
+// that fp16 has its eleven bits for those down to 2^-28 of the largest.
 constexpr float ATTN8_LIFT = 14.f;
 constexpr int ATTN8_MAX_BATCH = 2048;
 

@@ -19,8 +19,8 @@
 // of the token's largest value); infinities and NaN of its V stay out of the products (0 times them would reach rows
 // that do not see the token) and join their channel of the rows that see them at the end.
 // Bound: the softmax (the exponentials alone, 16 a clock and SM, take 2048 clocks for two 128x128 tiles; a row's 128
-// weights take its one thread about 2500).  Measured: 2048 tokens over 17200 keys, 16 heads of 64, 343 us (397 TFLOP/s);
-// 1024 tokens over 8000 keys, 32/8 heads of 128, 255 us.
+// weights take its one thread about 2500).  Measured: 2048 tokens over 17200 keys, 16 heads of 64, 338 us (403 TFLOP/s);
+// 1024 tokens over 8000 keys, 32/8 heads of 128, 257 us.
 #pragma once
 
 #include <type_traits>

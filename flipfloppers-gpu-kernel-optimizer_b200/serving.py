@@ -15,6 +15,7 @@ and raises on arguments the kernels do not take; there is no other implementatio
 behind it.  The operators' row counts and lengths are device tensors (int32), so
 that a step written with them can be captured in a CUDA graph and replayed with
 other values in them (``Int8Decoder`` counts on the host, and is not captured).
+All of it is for inference: results carry no autograd graph, whatever the inputs.
 """
 
 from __future__ import annotations
@@ -143,7 +144,8 @@ class PagedKV8:
 
         Row cu[b] + i of ``q`` is the token at position lens[b] - n + i of sequence b (n = cu[b+1] -
         cu[b] <= ``max_q_len``), appended already; it sees the keys up to its own.  A row with no key
-        gives zeros.  ``scale`` defaults to 1 / sqrt(D).  ``out`` may be q itself, and not overlap it
+        gives zeros.  Weights are rounded to fp16 before they meet V (2^-11 of each), scores, maxima and
+        sums are fp32.  ``scale`` defaults to 1 / sqrt(D).  ``out`` may be q itself, and not overlap it
         otherwise.  The same inputs give the same bits."""
         return _done(_module.attend(self._c, q, cu, lens, max_q_len, scale, out), "b200_kv8_attention")
 

@@ -365,6 +365,7 @@ int b200_kv8_read(const B200KvCache8* cache, const int* cu, const int* start, co
  * to its own; heads % kv_heads == 0, consecutive query heads share a key head.  A
  * row with no key (position < 0) gives zeros.  What is not finite in the newest block
  * reaches the rows that see it and no others (NaN, or the infinity in its channel).
+ * Weights are rounded to fp16 before they meet V, scores, maxima and sums are fp32.
  * max_q_len >= every n.  out may be q itself, and not overlap it otherwise.  No atomics:
  * the same inputs give the same bits. */
 size_t b200_kv8_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int max_q_len);
